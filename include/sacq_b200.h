@@ -302,6 +302,96 @@ SACQ_API int sacq_linear_a8_static_scratch(const sacq_layer_t* layer, const void
                                            void* y_out, int64_t ldy, void* stream);
 SACQ_API int64_t sacq_static_scratch_bytes(void);
 
+/* ---- the steps of a transformer block between its quantized projections ------------------------
+ * The reference leaves these to its framework (stock attention, rotary embedding and norms of the models that it
+ * patches); they are here so that a block runs on this library alone.  All tensors are bf16 device memory; strides and
+ * pitches are in elements, the innermost stride is 1.  No entry point allocates or synchronises. */
+
+/* Heads of a token: element (t, h, i) of `in` at t * in_token + h * in_head + i, of `out` likewise.  `out` may be `in`
+ * (same strides); otherwise the two may not overlap. */
+typedef struct sacq_head_rows {
+  const void* in;
+  void* out;
+  int64_t in_token, in_head, out_token, out_head;
+  int32_t heads;            /* 0: none, pointers may be null */
+  int32_t reserved;
+} sacq_head_rows;
+
+#define SACQ_ROTARY_HALF 0        /* pairs (i, i + rotary_dim / 2)   */
+#define SACQ_ROTARY_INTERLEAVED 1 /* pairs (2 i, 2 i + 1)            */
+
+typedef struct sacq_rotary_desc {
+  uint32_t struct_size;     /* sizeof(sacq_rotary_desc) */
+  int32_t layout;           /* SACQ_ROTARY_* */
+  sacq_head_rows q, k;
+  int64_t tokens;
+  int32_t head_dim, rotary_dim;   /* rotary_dim even, <= head_dim; the rest of a head is copied */
+  const void* positions;    /* [tokens], signed integers */
+  int32_t position_bytes;   /* 4 or 8 */
+  float amplitude;          /* multiplies cosine and sine */
+  const double* inv_freq;   /* [rotary_dim / 2] radians per position */
+} sacq_rotary_desc;
+
+/* Rotary positions of query and key heads in one launch:
+ *   (a, b) -> bf16( amplitude (a cos t - b sin t), amplitude (b cos t + a sin t) ),  t = position * inv_freq[i]
+ * Angles are made and reduced in double, the rest is fp32. */
+SACQ_API int sacq_rotate_heads(const sacq_rotary_desc* desc, void* stream);
+
+#define SACQ_NORM_NONE 0
+#define SACQ_NORM_RMS 1           /* x / sqrt(mean(x^2) + eps)         */
+#define SACQ_NORM_LAYER 2         /* (x - mean) / sqrt(var + eps)      */
+
+typedef struct sacq_residual_norm_desc {
+  uint32_t struct_size;     /* sizeof(sacq_residual_norm_desc) */
+  int32_t norm, post_norm;  /* SACQ_NORM_*; post_norm may be SACQ_NORM_NONE */
+  float eps, residual_scale;
+  uint32_t reserved;
+  int64_t M, K;
+  const void* branch;       /* [M, branch_pitch] output of the block */
+  const void* residual;     /* [M, residual_pitch] its input */
+  int64_t branch_pitch, residual_pitch;
+  const void *post_weight, *post_bias, *weight, *bias; /* [K] or null (no factor, no summand) */
+  const void *gate, *mod_scale, *mod_shift;            /* [K], or [vectors, K] with vector_rows; null: none */
+  const int32_t* vector_rows; /* [M] row of gate, mod_scale and mod_shift for each row, or null */
+  int64_t vectors;
+  void* residual_out;       /* [M, K]; may be `residual` if its pitch is K */
+  void* normalized_out;     /* [M, K] or null */
+  void* q_out;              /* [M, K] e4m3 bytes, or null */
+  float* scale_out;         /* [M], with q_out */
+} sacq_residual_norm_desc;
+
+/* The norms behind and before a block with its gate and residual scale, and the next projections' quantizer, in one launch:
+ *   r = residual_scale * residual + gate * (norm_post(branch) * post_weight + post_bias)
+ *   h = (norm(r) * weight + bias) * (1 + mod_scale) + mod_shift
+ * residual_out = bf16(r), normalized_out = bf16(h), scale = max|h| / 448 (1 for a row of zeros), q = e4m3(h / scale).
+ * Unlike the fused quantizers above nothing is rounded in between: h is made from the fp32 r and q from the fp32 h.
+ * A row whose vector_rows entry lies outside of [0, vectors) becomes NaN. */
+SACQ_API int sacq_residual_norm(const sacq_residual_norm_desc* desc, void* stream);
+
+typedef struct sacq_attention_desc {
+  uint32_t struct_size;     /* sizeof(sacq_attention_desc) */
+  int32_t causal;           /* query i of n sees keys up to i + (keys - n) */
+  const void *q, *k, *v;    /* [tokens_q, heads, head_dim], [tokens_k, kv_heads, head_dim] x 2 */
+  void* out;                /* like q; rows outside of every sequence are left as they are */
+  float* lse;               /* [tokens_q, heads] ln of the sum of exponentials, or null */
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head; /* strides */
+  int64_t tokens_q, tokens_k;
+  const int32_t *cu_q, *cu_k; /* [sequences + 1] first row of each sequence and the end of the last, device memory */
+  int32_t sequences, heads, kv_heads, head_dim; /* heads a multiple of kv_heads; head_dim <= 256 */
+  float scale;              /* positive */
+  uint32_t reserved;
+  void* workspace;          /* sacq_attention_workspace_bytes() bytes, 256-byte aligned; null if that is 0 */
+  int64_t workspace_bytes;
+} sacq_attention_desc;
+
+/* Softmax attention of packed sequences of different lengths, query heads in groups of heads / kv_heads:
+ *   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j)  over the keys that the query sees
+ * Scores, sums and the running maximum are fp32.  A query that sees no key has out = 0 and lse = -inf.  Offsets that leave the
+ * tensors or go backwards are cut to them.  What lies in keys and values that a query does not see, NaN included, does not
+ * reach its output. */
+SACQ_API int sacq_attention_packed(const sacq_attention_desc* desc, void* stream);
+SACQ_API int64_t sacq_attention_workspace_bytes(const sacq_attention_desc* desc);
+
 /* Forces a GEMM kernel (for tests and benchmarks): 0 = automatic, 1 = small-M kernel
  * (its own choice of variant), 2 = tensor-core kernel that splits K over clusters, 3 = small-M
  * CUDA-core variant, 4 = small-M warp-MMA variant, 5 = warp-MMA variant without shared-memory staging, 6 = warp-MMA variant that unpacks the indices in shared memory

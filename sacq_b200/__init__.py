@@ -8,30 +8,23 @@ from .packing import index_bits_for, index_window_bytes, pack_indices, pack_payl
 
 __all__ = [
     "PrecomputedPackedVectorCodebookLinear", "forward_shared", "linear_a8_multi", "quantize_rows", "act_quantize_rows", "modulate_quantize_rows", "layernorm_quantize_rows", "pack_indices", "unpack_indices",
-    "pack_payload", "index_bits_for", "index_window_bytes",
+    "pack_payload", "index_bits_for", "index_window_bytes", "attention_packed", "rotate_heads", "rotary_frequencies",
+    "residual_norm_quantize_rows",
 ]
 
 
+# public names that need the CUDA library, and the module each is in; looked up on first use
+_LAZY = {
+    "PrecomputedPackedVectorCodebookLinear": "linear", "forward_shared": "linear", "linear_a8_multi": "linear",
+    "layernorm_quantize_rows": "activation", "modulate_quantize_rows": "activation", "act_quantize_rows": "activation",
+    "quantize_rows": "activation", "residual_norm_quantize_rows": "activation", "attention_packed": "attention",
+    "rotate_heads": "rotary", "rotary_frequencies": "rotary",
+}
+
+
 def __getattr__(name):
-    if name == "PrecomputedPackedVectorCodebookLinear":
-        from .linear import PrecomputedPackedVectorCodebookLinear
-        return PrecomputedPackedVectorCodebookLinear
-    if name == "forward_shared":
-        from .linear import forward_shared
-        return forward_shared
-    if name == "linear_a8_multi":
-        from .linear import linear_a8_multi
-        return linear_a8_multi
-    if name == "layernorm_quantize_rows":
-        from .activation import layernorm_quantize_rows
-        return layernorm_quantize_rows
-    if name == "modulate_quantize_rows":
-        from .activation import modulate_quantize_rows
-        return modulate_quantize_rows
-    if name == "act_quantize_rows":
-        from .activation import act_quantize_rows
-        return act_quantize_rows
-    if name == "quantize_rows":
-        from .activation import quantize_rows
-        return quantize_rows
-    raise AttributeError(name)
+    if name not in _LAZY:
+        raise AttributeError(name)
+    from importlib import import_module
+    found = globals()[name] = getattr(import_module("." + _LAZY[name], __name__), name)   # from now on a plain name
+    return found

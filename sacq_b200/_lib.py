@@ -49,6 +49,41 @@ class LayerDesc(ctypes.Structure):
     ]
 
 
+class HeadRows(ctypes.Structure):
+    _fields_ = [("in_", ctypes.c_void_p), ("out", ctypes.c_void_p), ("in_token", ctypes.c_int64), ("in_head", ctypes.c_int64),
+                ("out_token", ctypes.c_int64), ("out_head", ctypes.c_int64), ("heads", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_uint32), ("layout", ctypes.c_int32), ("q", HeadRows), ("k", HeadRows),
+                ("tokens", ctypes.c_int64), ("head_dim", ctypes.c_int32), ("rotary_dim", ctypes.c_int32),
+                ("positions", ctypes.c_void_p), ("position_bytes", ctypes.c_int32), ("amplitude", ctypes.c_float),
+                ("inv_freq", ctypes.c_void_p)]
+
+
+class ResidualNormDesc(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_uint32), ("norm", ctypes.c_int32), ("post_norm", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("residual_scale", ctypes.c_float), ("reserved", ctypes.c_uint32),
+                ("M", ctypes.c_int64), ("K", ctypes.c_int64), ("branch", ctypes.c_void_p), ("residual", ctypes.c_void_p),
+                ("branch_pitch", ctypes.c_int64), ("residual_pitch", ctypes.c_int64), ("post_weight", ctypes.c_void_p),
+                ("post_bias", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+                ("gate", ctypes.c_void_p), ("mod_scale", ctypes.c_void_p), ("mod_shift", ctypes.c_void_p),
+                ("vector_rows", ctypes.c_void_p), ("vectors", ctypes.c_int64), ("residual_out", ctypes.c_void_p),
+                ("normalized_out", ctypes.c_void_p), ("q_out", ctypes.c_void_p), ("scale_out", ctypes.c_void_p)]
+
+
+class AttentionDesc(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_uint32), ("causal", ctypes.c_int32), ("q", ctypes.c_void_p), ("k", ctypes.c_void_p),
+                ("v", ctypes.c_void_p), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+                *((n, ctypes.c_int64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "out_token",
+                                                "out_head", "tokens_q", "tokens_k")),
+                ("cu_q", ctypes.c_void_p), ("cu_k", ctypes.c_void_p),
+                *((n, ctypes.c_int32) for n in ("sequences", "heads", "kv_heads", "head_dim")),
+                ("scale", ctypes.c_float), ("reserved", ctypes.c_uint32), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_int64)]
+
+
 _vp, _i64, _int = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
 _fp = ctypes.c_void_p  # float* passed as a raw device address
 
@@ -89,6 +124,10 @@ SIGNATURES = {
     "sacq_host_forward_scratch_bytes": (_i64, [_vp, _i64]),
     "sacq_linear_a8_static_scratch": (_int, [_vp, _vp, _fp, _i64, _vp, _i64, _vp]),
     "sacq_static_scratch_bytes": (_i64, []),
+    "sacq_rotate_heads": (_int, [ctypes.POINTER(RotaryDesc), _vp]),
+    "sacq_residual_norm": (_int, [ctypes.POINTER(ResidualNormDesc), _vp]),
+    "sacq_attention_packed": (_int, [ctypes.POINTER(AttentionDesc), _vp]),
+    "sacq_attention_workspace_bytes": (_i64, [ctypes.POINTER(AttentionDesc)]),
     "sacq_layer_set_kernel": (_int, [_vp, _int]),
     "sacq_layer_set_shard_of": (_int, [_vp, _i64]),
     "sacq_layer_kernel_for": (_int, [_vp, _i64]),

@@ -143,3 +143,87 @@ def layernorm_quantize_rows(x: torch.Tensor, weight: torch.Tensor | None = None,
                                                     s.data_ptr(), torch.cuda.current_stream().cuda_stream))
     q = q.view(torch.float8_e4m3fn)
     return (q, s, y) if return_normalized else (q, s)
+
+
+_NORMS = {None: 0, "rms": 1, "layer": 2}
+
+
+def residual_norm_quantize_rows(branch: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None,
+                                bias: torch.Tensor | None = None, *, norm: str = "rms", eps: float = 1e-6,
+                                post_norm: str | None = None, post_weight: torch.Tensor | None = None,
+                                post_bias: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                                residual_scale: float = 1.0, mod_scale: torch.Tensor | None = None,
+                                mod_shift: torch.Tensor | None = None, vector_rows: torch.Tensor | None = None,
+                                quantize: bool = True, return_normalized: bool = False):
+    """The norms behind and before a block, its gate and residual, and the next projections' quantizer in one launch
+    (``sacq_residual_norm``).  For the output ``branch`` of a block and its input ``residual``, bf16 ``[M, K]``::
+
+        r = residual_scale * residual + gate * (norm_post(branch) * post_weight + post_bias)
+        h = (norm(r) * weight + bias) * (1 + mod_scale) + mod_shift
+
+    ``norm``: ``"rms"`` or ``"layer"``, ``post_norm``: one of them, or ``None`` for the branch as it is; weights and biases are bf16 ``[K]`` or
+    ``None``.  ``gate``, ``mod_scale`` and ``mod_shift`` are bf16 ``[K]``, or ``[R, K]`` with ``vector_rows`` (int32 ``[M]``, the row of them that
+    each token takes; one outside of ``[0, R)`` makes its token NaN).  Returns ``(r, q, scale)`` with ``r`` in bf16 and the FP8 rows of ``h``, with
+    ``return_normalized`` ``(r, q, scale, h)``, or with ``quantize=False`` ``(r, h)``.  Sums and everything in between are fp32, and each
+    result is rounded once: ``q`` is made from the fp32 ``h``, not from its bf16 rounding as in ``layernorm_quantize_rows``."""
+    if norm not in ("rms", "layer") or post_norm not in _NORMS:
+        raise ValueError(f"unknown norm {norm!r} or post_norm {post_norm!r}")
+    args = (_NORMS[norm], _NORMS[post_norm], float(eps), float(residual_scale), bool(quantize), bool(return_normalized))
+    made = _lib.native().residual_norm_quantize_rows(branch, residual, weight, bias, post_weight, post_bias, gate, mod_scale,
+                                                     mod_shift, vector_rows, *args)
+    if made is not None:
+        return made
+    from .attention import refuse_grad
+    for t, what in ((branch, "branch"), (residual, "residual")):
+        if not isinstance(t, torch.Tensor) or t.ndim != 2 or t.dtype != torch.bfloat16 or not t.is_cuda:
+            raise TypeError(f"{what} must be a 2-D bfloat16 CUDA tensor")
+    if branch.shape != residual.shape or branch.device != residual.device:
+        raise ValueError("branch and residual must have one shape and device")
+    m, k = branch.shape
+    vectors = {"weight": weight, "bias": bias, "post_weight": post_weight, "post_bias": post_bias}
+    tables = {"gate": gate, "mod_scale": mod_scale, "mod_shift": mod_shift}
+    refuse_grad("residual_norm_quantize_rows", branch, residual, *vectors.values(), *tables.values())
+    if post_norm is None and (post_weight is not None or post_bias is not None):
+        raise ValueError("post_weight and post_bias need a post_norm")
+    if (mod_scale is None) != (mod_shift is None):
+        raise ValueError("modulation needs both its scale and its shift")
+    if not eps >= 0.0:
+        raise ValueError("eps must be non-negative")
+    for name, t in {**vectors, **tables}.items():
+        if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.device != branch.device):
+            raise TypeError(f"{name} must be a bfloat16 tensor on branch's device")
+    for name, t in vectors.items():
+        if t is not None:
+            if t.numel() != k:
+                raise ValueError(f"{name} must have {k} elements")
+            vectors[name] = t.reshape(-1).contiguous()
+    rows = None
+    for name, t in tables.items():
+        if t is None:
+            continue
+        if vector_rows is None:
+            if t.numel() != k:
+                raise ValueError(f"{name} must have {k} elements, or rows of them with vector_rows")
+            tables[name] = t.reshape(-1).contiguous()
+        else:
+            if t.ndim != 2 or t.shape[1] != k or t.shape[0] == 0 or (rows is not None and t.shape[0] != rows):
+                raise ValueError(f"{name} must be [R, {k}], with one R for all")
+            rows = t.shape[0]
+            tables[name] = t.contiguous()
+    if vector_rows is not None:
+        if rows is None:
+            raise ValueError("vector_rows without a gate or a modulation")
+        if not isinstance(vector_rows, torch.Tensor) or vector_rows.dtype != torch.int32 or vector_rows.device != branch.device:
+            raise TypeError("vector_rows must be an int32 tensor on branch's device")
+        if vector_rows.numel() != m:
+            raise ValueError("vector_rows must have one entry per row")
+        vector_rows = vector_rows.reshape(-1).contiguous()
+    branch, residual = (t if t.stride(1) == 1 and t.stride(0) >= k else t.contiguous() for t in (branch, residual))
+    if m == 0 or k == 0:
+        y = torch.empty_like(branch)
+        q, s = torch.empty((m, k), dtype=torch.float8_e4m3fn, device=y.device), torch.ones((m, 1), device=y.device)
+        return (y, torch.empty_like(y)) if not quantize else (y, q, s, torch.empty_like(y)) if return_normalized else (y, q, s)
+    made = _lib.native().residual_norm_quantize_rows(branch, residual, *vectors.values(), *tables.values(), vector_rows, *args)
+    if made is None:
+        raise ValueError("residual_norm_quantize_rows: unsupported arguments")
+    return made

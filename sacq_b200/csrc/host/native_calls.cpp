@@ -17,12 +17,15 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <optional>
@@ -491,6 +494,247 @@ PyObject* py_layernorm_quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n
   NATIVE_CATCH
 }
 
+// ---------------------------------------------------------------- the steps between projections
+// Whether autograd would expect a backward pass through this call: refused by the general route.
+bool wants_grad(const at::Tensor& t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
+
+// bf16 [tokens, heads, dim] with unit inner stride and strides that go forwards
+const at::Tensor* heads_of(PyObject* o, int dev) {
+  const at::Tensor* t = tensor_of(o);
+  if (t == nullptr || t->scalar_type() != at::kBFloat16 || t->dim() != 3 || !t->is_cuda() || (dev >= 0 && t->get_device() != dev) ||
+      (t->stride(2) != 1 && t->size(2) > 1) || wants_grad(*t))
+    return nullptr;
+  return t;
+}
+
+// Bytes between the first and the last element
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  auto end = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return (const char*)t.data_ptr() + (last + 1) * t.element_size();
+  };
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  return (const char*)a.data_ptr() < end(b) && (const char*)b.data_ptr() < end(a);
+}
+
+// overlaps(a, (b, ...))
+PyObject* py_overlaps(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NATIVE_TRY
+  const at::Tensor* t = n == 2 ? tensor_of(a[0]) : nullptr;
+  if (t == nullptr || !PyTuple_Check(a[1])) Py_RETURN_FALSE;
+  for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(a[1]); ++i) {
+    const at::Tensor* b = tensor_of(PyTuple_GET_ITEM(a[1], i));
+    if (b != nullptr && overlap(*t, *b)) Py_RETURN_TRUE;
+  }
+  Py_RETURN_FALSE;
+  NATIVE_CATCH
+}
+
+PyObject* tuple_of(std::initializer_list<at::Tensor> list) {
+  PyObject* t = PyTuple_New((Py_ssize_t)list.size());
+  Py_ssize_t i = 0;
+  for (const at::Tensor& x : list) {
+    PyObject* o = t == nullptr ? nullptr : x.defined() ? THPVariable_Wrap(x) : Py_NewRef(Py_None);
+    if (o == nullptr) {
+      Py_XDECREF(t);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(t, i++, o);
+  }
+  return t;
+}
+
+bool offsets_of(const at::Tensor* t, int dev) {
+  return t != nullptr && t->scalar_type() == at::kInt && on_device(*t, dev) && t->dim() == 1 && t->numel() >= 1 && t->is_contiguous();
+}
+
+// attention_packed(q, k, v, cu_q, cu_k, causal, scale, out, return_lse)
+PyObject* py_attention_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NATIVE_TRY
+  const at::Tensor* q = n == 9 ? heads_of(a[0], -1) : nullptr;
+  if (q == nullptr) Py_RETURN_NONE;
+  const int dev = q->get_device();
+  const at::Tensor *k = heads_of(a[1], dev), *v = heads_of(a[2], dev), *cu_q = tensor_of(a[3]),
+                   *cu_k = a[4] == Py_None ? cu_q : tensor_of(a[4]);
+  if (k == nullptr || v == nullptr || k->sizes() != v->sizes() || !offsets_of(cu_q, dev) || !offsets_of(cu_k, dev) ||
+      cu_q->numel() != cu_k->numel())
+    Py_RETURN_NONE;
+  const int64_t h = q->size(1), d = q->size(2), hk = k->size(1);
+  if (d < 1 || d > 256 || h < 1 || hk < 1 || h % hk != 0 || k->size(2) != d || h > 65536) Py_RETURN_NONE;
+  double scale = 1.0 / std::sqrt((double)d);
+  if (a[6] != Py_None) {
+    scale = PyFloat_AsDouble(a[6]);
+    if (PyErr_Occurred()) PyErr_Clear();
+    if (!(scale > 0.0 && (float)scale > 0.f && std::isfinite((float)scale))) Py_RETURN_NONE;
+  }
+  Target at_(dev);
+  at::Tensor out;
+  if (a[7] == Py_None) {
+    out = new_tensor({q->size(0), h, d}, at::kBFloat16, dev);
+  } else {
+    const at::Tensor* o = heads_of(a[7], dev);
+    if (o == nullptr || o->sizes() != q->sizes() || overlap(*o, *q) || overlap(*o, *k) || overlap(*o, *v)) Py_RETURN_NONE;
+    out = *o;
+  }
+  const bool want_lse = a[8] == Py_True;
+  at::Tensor lse, ws;
+  if (want_lse) lse = new_tensor({q->size(0), h}, at::kFloat, dev);
+  sacq_attention_desc c = {};
+  c.struct_size = sizeof(c);
+  c.causal = a[5] == Py_True;
+  c.q = q->data_ptr();
+  c.k = k->data_ptr();
+  c.v = v->data_ptr();
+  c.out = out.data_ptr();
+  c.lse = want_lse ? (float*)lse.data_ptr() : nullptr;
+  c.q_token = q->stride(0); c.q_head = q->stride(1);
+  c.k_token = k->stride(0); c.k_head = k->stride(1);
+  c.v_token = v->stride(0); c.v_head = v->stride(1);
+  c.out_token = out.stride(0); c.out_head = out.stride(1);
+  c.tokens_q = q->size(0); c.tokens_k = k->size(0);
+  c.cu_q = (const int32_t*)cu_q->data_ptr();
+  c.cu_k = (const int32_t*)cu_k->data_ptr();
+  c.sequences = (int32_t)(cu_q->numel() - 1);
+  c.heads = (int32_t)h;
+  c.kv_heads = (int32_t)hk;
+  c.head_dim = (int32_t)d;
+  c.scale = (float)scale;
+  // partial results belong to the call: a captured graph keeps its own
+  c.workspace_bytes = sacq_attention_workspace_bytes(&c);
+  if (c.workspace_bytes < 0) return raise_status((int)c.workspace_bytes);
+  if (c.workspace_bytes > 0) {
+    ws = new_tensor({c.workspace_bytes}, at::kByte, dev);
+    c.workspace = ws.data_ptr();
+  }
+  const int rc = sacq_attention_packed(&c, at_.stream);
+  if (rc != 0) return raise_status(rc);
+  if (want_lse) return pair_of(std::move(out), std::move(lse));
+  return THPVariable_Wrap(std::move(out));
+  NATIVE_CATCH
+}
+
+bool fill_heads(const at::Tensor* x, PyObject* out_obj, int dev, sacq_head_rows& r, at::Tensor& out) {
+  if (out_obj == Py_None) {
+    out = new_tensor(x->sizes(), at::kBFloat16, dev);
+  } else {
+    const at::Tensor* o = heads_of(out_obj, dev);
+    if (o == nullptr || o->sizes() != x->sizes()) return false;
+    const bool same = o->data_ptr() == x->data_ptr() && o->strides() == x->strides();
+    if (!same && overlap(*o, *x)) return false;
+    out = *o;
+  }
+  r.in = x->data_ptr();
+  r.out = out.data_ptr();
+  r.in_token = x->stride(0); r.in_head = x->stride(1);
+  r.out_token = out.stride(0); r.out_head = out.stride(1);
+  r.heads = (int32_t)x->size(1);
+  return true;
+}
+
+// rotate_heads(q, k, positions, inv_freq, layout, amplitude, q_out, k_out)
+PyObject* py_rotate_heads(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NATIVE_TRY
+  const at::Tensor* q = n == 8 ? heads_of(a[0], -1) : nullptr;
+  if (q == nullptr) Py_RETURN_NONE;
+  const int dev = q->get_device();
+  const at::Tensor *k = nullptr, *pos = tensor_of(a[2]), *freq = tensor_of(a[3]);
+  if (a[1] != Py_None) {
+    k = heads_of(a[1], dev);
+    if (k == nullptr || k->size(0) != q->size(0) || k->size(2) != q->size(2)) Py_RETURN_NONE;
+  } else if (a[7] != Py_None) {
+    Py_RETURN_NONE;
+  }
+  if (pos == nullptr || freq == nullptr || !on_device(*pos, dev) || !on_device(*freq, dev) || pos->dim() != 1 || freq->dim() != 1 ||
+      !pos->is_contiguous() || !freq->is_contiguous() || pos->numel() != q->size(0) ||
+      (pos->scalar_type() != at::kInt && pos->scalar_type() != at::kLong) || freq->scalar_type() != at::kDouble ||
+      freq->numel() < 1 || 2 * freq->numel() > q->size(2))
+    Py_RETURN_NONE;
+  Target at_(dev);
+  sacq_rotary_desc c = {};
+  c.struct_size = sizeof(c);
+  at::Tensor q_out, k_out;
+  if (!fill_heads(q, a[6], dev, c.q, q_out) || (k != nullptr && !fill_heads(k, a[7], dev, c.k, k_out))) Py_RETURN_NONE;
+  c.layout = (int32_t)PyLong_AsLong(a[4]);
+  c.tokens = q->size(0);
+  c.head_dim = (int32_t)q->size(2);
+  c.rotary_dim = (int32_t)(2 * freq->numel());
+  c.positions = pos->data_ptr();
+  c.position_bytes = pos->scalar_type() == at::kLong ? 8 : 4;
+  c.amplitude = (float)PyFloat_AsDouble(a[5]);
+  c.inv_freq = (const double*)freq->data_ptr();
+  if (PyErr_Occurred()) return nullptr;
+  const int rc = sacq_rotate_heads(&c, at_.stream);
+  return rc == 0 ? tuple_of({q_out, k_out}) : raise_status(rc);
+  NATIVE_CATCH
+}
+
+// residual_norm_quantize_rows(branch, residual, weight, bias, post_weight, post_bias, gate, mod_scale, mod_shift, vector_rows, norm,
+// post_norm, eps, residual_scale, quantize, return_normalized)
+PyObject* py_residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NATIVE_TRY
+  const at::Tensor *x = n == 16 ? quantizer_input(a[0]) : nullptr, *res = n == 16 ? tensor_of(a[1]) : nullptr;
+  if (x == nullptr || res == nullptr || res->dim() != 2 || res->sizes() != x->sizes()) Py_RETURN_NONE;
+  const int dev = x->get_device();
+  const int64_t m = x->size(0), k = x->size(1);
+  if (!bf16_rows(*res, dev) || wants_grad(*x) || wants_grad(*res)) Py_RETURN_NONE;
+  if ((m > 1 && (x->stride(0) < k || res->stride(0) < k))) Py_RETURN_NONE;
+  sacq_residual_norm_desc c = {};
+  c.struct_size = sizeof(c);
+  const void** vec[4] = {&c.weight, &c.bias, &c.post_weight, &c.post_bias};
+  for (int i = 0; i < 4; ++i) {
+    if (!vector_or_none(a[2 + i], k, dev, vec[i])) Py_RETURN_NONE;
+    if (a[2 + i] != Py_None && wants_grad(*tensor_of(a[2 + i]))) Py_RETURN_NONE;
+  }
+  const at::Tensor* rows = a[9] == Py_None ? nullptr : tensor_of(a[9]);
+  if (a[9] != Py_None && (rows == nullptr || rows->scalar_type() != at::kInt || !on_device(*rows, dev) || rows->numel() != m ||
+                          !rows->is_contiguous()))
+    Py_RETURN_NONE;
+  const void** table[3] = {&c.gate, &c.mod_scale, &c.mod_shift};
+  for (int i = 0; i < 3; ++i) {
+    const at::Tensor* t = a[6 + i] == Py_None ? nullptr : tensor_of(a[6 + i]);
+    if (a[6 + i] == Py_None) continue;
+    if (t == nullptr || t->scalar_type() != at::kBFloat16 || !on_device(*t, dev) || !t->is_contiguous() || wants_grad(*t)) Py_RETURN_NONE;
+    if (rows == nullptr ? t->numel() != k : (t->dim() != 2 || t->size(1) != k || t->size(0) < 1)) Py_RETURN_NONE;
+    if (rows != nullptr && c.vectors != 0 && c.vectors != t->size(0)) Py_RETURN_NONE;
+    if (rows != nullptr) c.vectors = t->size(0);
+    *table[i] = t->data_ptr();
+  }
+  if (rows != nullptr && c.vectors == 0) Py_RETURN_NONE;
+  c.norm = (int32_t)PyLong_AsLong(a[10]);
+  c.post_norm = (int32_t)PyLong_AsLong(a[11]);
+  c.eps = (float)PyFloat_AsDouble(a[12]);
+  c.residual_scale = (float)PyFloat_AsDouble(a[13]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!(c.eps >= 0.f) || (c.mod_scale == nullptr) != (c.mod_shift == nullptr) ||
+      (c.post_norm == SACQ_NORM_NONE && (c.post_weight || c.post_bias)))
+    Py_RETURN_NONE;
+  const bool quantize = a[14] == Py_True, want_h = !quantize || a[15] == Py_True;
+  Target at_(dev);
+  at::Tensor r = new_tensor({m, k}, at::kBFloat16, dev), h, q, s;
+  if (want_h) h = new_tensor({m, k}, at::kBFloat16, dev);
+  if (quantize) {
+    Encoded e(m, k, false, dev);
+    q = std::move(e.q);
+    s = std::move(e.s);
+    c.q_out = q.data_ptr();
+    c.scale_out = (float*)s.data_ptr();
+  }
+  c.M = m;
+  c.K = k;
+  c.branch = x->data_ptr();
+  c.residual = res->data_ptr();
+  c.branch_pitch = m > 1 ? x->stride(0) : k;
+  c.residual_pitch = m > 1 ? res->stride(0) : k;
+  c.vector_rows = rows ? (const int32_t*)rows->data_ptr() : nullptr;
+  c.residual_out = r.data_ptr();
+  c.normalized_out = want_h ? h.data_ptr() : nullptr;
+  const int rc = sacq_residual_norm(&c, at_.stream);
+  if (rc != 0) return raise_status(rc);
+  return !quantize ? tuple_of({r, h}) : want_h ? tuple_of({r, q, s, h}) : tuple_of({r, q, s});
+  NATIVE_CATCH
+}
+
 // ---------------------------------------------------------------- several layers on one input
 constexpr int kMostSiblings = 16;
 
@@ -617,6 +861,10 @@ PyMethodDef module_methods[] = {
     {"act_quantize_rows", (PyCFunction)(void*)py_act_quantize_rows, METH_FASTCALL, nullptr},
     {"modulate_quantize_rows", (PyCFunction)(void*)py_modulate_quantize_rows, METH_FASTCALL, nullptr},
     {"layernorm_quantize_rows", (PyCFunction)(void*)py_layernorm_quantize_rows, METH_FASTCALL, nullptr},
+    {"attention_packed", (PyCFunction)(void*)py_attention_packed, METH_FASTCALL, nullptr},
+    {"rotate_heads", (PyCFunction)(void*)py_rotate_heads, METH_FASTCALL, nullptr},
+    {"residual_norm_quantize_rows", (PyCFunction)(void*)py_residual_norm, METH_FASTCALL, nullptr},
+    {"overlaps", (PyCFunction)(void*)py_overlaps, METH_FASTCALL, nullptr},
     {"linear_a8_multi", (PyCFunction)(void*)py_linear_a8_multi, METH_FASTCALL, nullptr},
     {"forward_shared", (PyCFunction)(void*)py_forward_shared, METH_FASTCALL, nullptr},
     {"workspace", py_workspace, METH_VARARGS, nullptr},

@@ -1,0 +1,557 @@
+"""Attention over packed sequences, rotary positions and the norms around a block against plain float64 evaluations.
+
+Tolerances are sums of the roundings a kernel makes: half a step of a bf16 result or weight is 2^-8 of the value, of an fp32
+operation 2^-24, of e4m3 2^-4; a sum of n fp32 terms is off by at most n 2^-24 of the sum of their magnitudes."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF, F32 = 2.0 ** -8, 2.0 ** -24
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.fixture(autouse=True)
+def _needs_cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(gen, *shape, at=0.0, by=1.0):
+    return (torch.randn(*shape, generator=gen, device="cuda") * by + at).to(torch.bfloat16)
+
+
+def _offsets(lengths):
+    return torch.tensor([0] + list(lengths), dtype=torch.int64).cumsum(0).to(torch.int32).cuda()
+
+
+# ----------------------------------------------------------------------------- attention
+
+def _attention_reference(q, k, v, lq, lk, causal, scale=None):
+    """(out, lse, bound of out, bound of lse) in float64, sequence by sequence.  Only keys that a query sees are looked at."""
+    d, g = q.shape[2], q.shape[1] // k.shape[1]
+    scale = d ** -0.5 if scale is None else scale
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    lse = torch.full(q.shape[:2], -INF, dtype=torch.float64, device=q.device)
+    tol, tol_lse = torch.zeros_like(out), torch.zeros_like(lse)
+    aq = ak = 0
+    for nq, nk in zip(lq, lk):
+        if nq and nk:
+            qs = q[aq:aq + nq].double().transpose(0, 1)
+            ks, vs = (t[ak:ak + nk].double().transpose(0, 1).repeat_interleave(g, 0) for t in (k, v))
+            s = qs @ ks.transpose(1, 2) * scale
+            # a score is a sum of d products in fp32, scaled and shifted by the maximum; exp and its argument: 2^-20
+            off = (qs.abs() @ ks.abs().transpose(1, 2) * scale) * (d + 8) * F32
+            seen = torch.ones(nq, nk, dtype=torch.bool, device=q.device)
+            if causal:
+                seen = seen.tril(nk - nq)
+            s = s.masked_fill(~seen, -INF)
+            off = (off + s.abs() * 4 * F32).masked_fill(~seen, 0.0)
+            le = torch.logsumexp(s, 2)
+            p = (s - le.masked_fill(le == -INF, 0.0)[..., None]).exp()
+            spread = (p @ vs.abs()).transpose(0, 1)                     # sum p |v|
+            worst = off.amax(2).transpose(0, 1)[..., None]
+            o = p @ vs
+            o = o.transpose(0, 1)
+            out[aq:aq + nq], lse[aq:aq + nq] = o, le.transpose(0, 1)
+            # weights rounded to bf16, fp32 sums of nk terms, errors of the scores on weights and their sum, the result rounded to bf16
+            rel = BF + nk * F32 + 2 * worst + 2.0 ** -20
+            tol[aq:aq + nq] = spread.nan_to_num(0.0) * rel * 1.01 + o.abs().nan_to_num(0.0) * BF * 1.01 + 1e-30
+            tol_lse[aq:aq + nq] = worst[..., 0] + (nk + 8) * F32 + 2.0 ** -20 + le.transpose(0, 1).abs().nan_to_num(0.0, posinf=0.0) * 4 * F32
+        aq, ak = aq + nq, ak + nk
+    return out, lse, tol, tol_lse
+
+
+def _check_attention(got, lse, ref):
+    out, le, tol, tol_le = ref
+    got, lse = got.double(), lse.double()
+    assert bool(torch.isfinite(got).all())
+    bad = (got - out).abs() - tol
+    assert float(bad.max()) <= 0, (float(bad.max()), (bad > 0).nonzero()[:4].tolist())
+    none = le == -INF
+    assert torch.equal(lse == -INF, none) and bool((got[none] == 0).all())
+    off = (lse - le).abs()[~none] - tol_le[~none]
+    assert off.numel() == 0 or float(off.max()) <= 0, float(off.max())
+
+
+def _attend(lq, lk, heads, kv_heads, dim, causal, seed=0, by=1.5, scale=None):
+    from sacq_b200 import attention_packed
+    gen = _gen(seed)
+    q = _randn(gen, sum(lq), heads, dim, by=by)
+    k, v = (_randn(gen, sum(lk), kv_heads, dim, by=by) for _ in range(2))
+    got, lse = attention_packed(q, k, v, _offsets(lq), _offsets(lk), causal=causal, scale=scale, return_lse=True)
+    assert got.dtype == torch.bfloat16 and got.shape == q.shape and lse.dtype == torch.float32
+    _check_attention(got, lse, _attention_reference(q, k, v, lq, lk, causal, scale))
+
+
+@pytest.mark.parametrize("causal", (False, True))
+@pytest.mark.parametrize("lengths", ([1], [2, 1, 3], [16], [63, 64, 65], [127, 1, 128, 129], [255, 256, 257], [300, 0, 41], [513, 700]))
+def test_attention_of_a_prompt(lengths, causal):
+    _attend(lengths, lengths, 4, 2, 128, causal)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", ((12, 12, 128), (16, 16, 64), (8, 1, 128), (6, 2, 96), (9, 3, 64), (4, 4, 80), (7, 1, 8), (12, 1, 16),
+                                                (128, 1, 64), (5, 5, 72), (2, 1, 112), (3, 1, 36), (2, 2, 200), (1, 1, 1), (4, 2, 256)))
+@pytest.mark.parametrize("causal", (False, True))
+def test_attention_head_layouts(heads, kv_heads, dim, causal):
+    _attend([70, 150, 5], [70, 150, 5], heads, kv_heads, dim, causal)
+
+
+@pytest.mark.parametrize("lq,lk", (([16, 16], [300, 270]), ([1, 1, 1], [1, 500, 4097]), ([1], [20000]), ([3, 7], [130, 128]), ([200, 5], [7, 130]),
+                                   ([130, 4, 9], [0, 0, 40]), ([40, 0, 3], [30, 50, 0]), ([150], [1]), ([2, 1, 300], [6000, 31, 2500])))
+@pytest.mark.parametrize("causal", (False, True))
+def test_attention_to_keys_of_other_lengths(lq, lk, causal):
+    # causal with fewer keys than queries: the first queries see none
+    _attend(lq, lk, 4, 2, 128, causal)
+    _attend(lq, lk, 3, 3, 64, causal, seed=1)
+
+
+def test_attention_of_many_sequences():
+    lengths = [(7 * i) % 40 for i in range(300)]
+    _attend(lengths, lengths, 2, 1, 64, True)
+    _attend([1] * 300, [(37 * i) % 700 for i in range(300)], 4, 2, 128, True)
+
+
+@pytest.mark.parametrize("by", (0.01, 6.0, 40.0))
+def test_attention_of_flat_and_peaked_scores(by):
+    _attend([200, 77], [200, 77], 4, 2, 128, True, by=by)
+    _attend([200, 77], [1200, 77], 2, 2, 64, False, by=by)
+
+
+def test_attention_rising_scores():
+    """Each tile of keys outdoes the ones in front of it, so that every step rescales what it has."""
+    from sacq_b200 import attention_packed
+    gen = _gen(3)
+    n = 700
+    q, k, v = (_randn(gen, n, 2, 128) for _ in range(3))
+    k = (k.float() * 0.1 + q[:1].float() * torch.linspace(0, 4, n, device="cuda")[:, None, None]).to(torch.bfloat16)
+    q = (q[:1].float() + q.float() * 0.05).to(torch.bfloat16)
+    for causal in (False, True):
+        got, lse = attention_packed(q, k, v, _offsets([n]), causal=causal, return_lse=True)
+        _check_attention(got, lse, _attention_reference(q, k, v, [n], [n], causal))
+
+
+@pytest.mark.parametrize("scale", (1.0, 0.3, 1e-4))
+def test_attention_scale(scale):
+    _attend([90, 33], [90, 33], 2, 2, 64, True, by=1.0, scale=scale)
+
+
+@pytest.mark.parametrize("dim", (64, 128))
+def test_attention_reads_views_where_they_lie(dim):
+    from sacq_b200 import attention_packed
+    gen = _gen(4)
+    lengths = [140, 33, 250]
+    t, h, hk = sum(lengths), 6, 2
+    fused = _randn(gen, t, (h + 2 * hk) * dim + 8)
+    q, k, v = (fused[:, a * dim:(a + n) * dim].view(t, n, dim) for a, n in ((0, h), (h, hk), (h + hk, hk)))
+    out = torch.full((t + 5, h, 2 * dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    got, lse = attention_packed(q, k, v, _offsets(lengths), causal=True, out=out[2:t + 2, :, dim:], return_lse=True)
+    assert got.data_ptr() == out[2:t + 2, :, dim:].data_ptr()
+    _check_attention(got, lse, _attention_reference(q, k, v, lengths, lengths, True))
+    assert bool((out[:2] == 7).all()) and bool((out[t + 2:] == 7).all()) and bool((out[..., :dim] == 7).all())
+    # heads first, an inner stride that is not one, a head stride that is not a multiple of 8 elements
+    for make in (lambda x: x.transpose(0, 1).contiguous().transpose(0, 1), lambda x: x.transpose(1, 2).contiguous().transpose(1, 2),
+                 lambda x: torch.nn.functional.pad(x, (0, 3))[..., :dim], lambda x: torch.nn.functional.pad(x.reshape(t, -1), (1, 0))[:, 1:].view(x.shape)):
+        again = attention_packed(make(q), make(k), make(v), _offsets(lengths), causal=True)
+        ref = _attention_reference(q, k, v, lengths, lengths, True)
+        assert float(((again.double() - ref[0]).abs() - ref[2]).max()) <= 0
+    # one key-value row for every token
+    one = k[:1].expand(t, hk, dim)
+    again, lse = attention_packed(q, one, one, _offsets(lengths), causal=True, return_lse=True)
+    _check_attention(again, lse, _attention_reference(q, one, one, lengths, lengths, True))
+
+
+@pytest.mark.parametrize("heads,dim", (((4, 2), 128), ((2, 2), 64), ((2, 1), 36)))
+@pytest.mark.parametrize("value", (NAN, INF, -INF))
+def test_attention_keeps_what_is_not_seen_out(value, heads, dim):
+    """Rows of no sequence, of other sequences and of later tokens may hold anything."""
+    from sacq_b200 import attention_packed
+    gen = _gen(5)
+    lengths = [130, 3, 60]
+    front, behind = 9, 100
+    t = front + sum(lengths) + behind
+    q, k, v = (_randn(gen, t, n, dim) for n in (heads[0], heads[1], heads[1]))
+    cu = (_offsets(lengths) + front).to(torch.int32)
+    real = slice(front, t - behind)
+    ref = _attention_reference(q[real], k[real], v[real], lengths, lengths, True)
+    for x in (q, k, v):
+        x[:front], x[t - behind:] = value, value
+    out = torch.full_like(q, 3.0)
+    lse = attention_packed(q, k, v, cu, causal=True, out=out, return_lse=True)[1]
+    _check_attention(out[real], lse[real], ref)
+    assert bool((out[:front] == 3).all()) and bool((out[t - behind:] == 3).all())
+    # the middle sequence and the last tokens of the first
+    k2, v2 = k.clone(), v.clone()
+    hidden = slice(front + 120, front + 133)
+    k2[hidden], v2[hidden] = value, value
+    attention_packed(q, k2, v2, cu, causal=True, out=out)
+    clean = list(range(0, 120)) + list(range(133, sum(lengths)))
+    bad = (out[real][clean].double() - ref[0][clean]).abs() - ref[2][clean]
+    assert float(bad.max()) <= 0
+
+
+def test_attention_of_infinities_that_are_seen():
+    """A visible NaN or infinity reaches the rows that see it as it does in the formula."""
+    from sacq_b200 import attention_packed
+    gen = _gen(6)
+    q, k, v = (_randn(gen, 40, 1, 64) for _ in range(3))
+    v[30, 0, 5], v[35, 0, 6] = INF, NAN
+    out = attention_packed(q, k, v, _offsets([40]), causal=True)
+    assert bool(torch.isfinite(out[:30]).all())
+    assert bool((out[30:, 0, 5] == INF).all()) and bool(torch.isfinite(out[30:35, 0, 6]).all()) and bool(out[35:, 0, 6].isnan().all())
+    k[20] = NAN
+    out = attention_packed(q, k, v, _offsets([40]), causal=True)
+    assert bool(torch.isfinite(out[:20]).all()) and bool(out[20:].isnan().all())
+
+
+def test_attention_is_the_same_twice_and_does_not_depend_on_the_batch():
+    from sacq_b200 import attention_packed
+    gen = _gen(7)
+    lengths = [300, 120, 4, 700]
+    q, k, v = (_randn(gen, sum(lengths), n, 128) for n in (8, 4, 4))
+    a, b = (attention_packed(q, k, v, _offsets(lengths), causal=True) for _ in range(2))
+    assert torch.equal(a, b)
+    at = 0
+    for n in lengths:
+        one = attention_packed(q[at:at + n], k[at:at + n], v[at:at + n], _offsets([n]), causal=True)
+        ref = _attention_reference(q[at:at + n], k[at:at + n], v[at:at + n], [n], [n], True)
+        assert float(((one.double() - ref[0]).abs() - ref[2]).max()) <= 0
+        assert float((one.double() - a[at:at + n].double()).abs().sub(2 * ref[2]).max()) <= 0
+        at += n
+
+
+def test_attention_offsets_that_leave_the_tensors():
+    """Offsets are cut to the tensors, and a sequence that ends in front of its beginning is empty."""
+    from sacq_b200 import attention_packed
+    gen = _gen(8)
+    q, k, v = (_randn(gen, 100, 2, 64) for _ in range(3))
+    cu = torch.tensor([-5, 40, 1000], dtype=torch.int32, device="cuda")
+    out, lse = attention_packed(q, k, v, cu, return_lse=True)
+    _check_attention(out, lse, _attention_reference(q, k, v, [40, 60], [40, 60], False))
+    out = torch.full_like(q, 2.0)
+    attention_packed(q, k, v, torch.tensor([60, 20, 100], dtype=torch.int32, device="cuda"), out=out)
+    ref = _attention_reference(q[20:], k[20:], v[20:], [80], [80], False)
+    assert float(((out[20:].double() - ref[0]).abs() - ref[2]).max()) <= 0
+    assert bool((out[:20] == 2).all())
+
+
+def test_attention_empty_calls():
+    from sacq_b200 import attention_packed
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    assert attention_packed(z(0, 4, 64), z(0, 2, 64), z(0, 2, 64), _offsets([])).shape == (0, 4, 64)
+    out, lse = attention_packed(z(5, 4, 64) + 1, z(0, 2, 64), z(0, 2, 64), _offsets([5]), _offsets([0]), return_lse=True)
+    assert bool((out == 0).all()) and bool((lse == -INF).all())
+    out = torch.full((5, 4, 64), 9.0, dtype=torch.bfloat16, device="cuda")
+    attention_packed(z(5, 4, 64), z(3, 2, 64), z(3, 2, 64), _offsets([]), out=out)
+    assert bool((out == 9).all())
+
+
+# ----------------------------------------------------------------------------- rotary positions
+
+def _rotary_reference(x, positions, inv_freq, layout, amplitude):
+    r = 2 * inv_freq.numel()
+    x = x.double()
+    angle = positions.double()[:, None, None] * inv_freq
+    c, s = angle.cos() * amplitude, angle.sin() * amplitude
+    i = torch.arange(r // 2, device=x.device)
+    first, second = (i, i + r // 2) if layout == "half" else (2 * i, 2 * i + 1)
+    y, tol = x.clone(), torch.zeros_like(x)
+    a, b = x[..., first], x[..., second]
+    y[..., first], y[..., second] = a * c - b * s, b * c + a * s
+    # the angle rounded to 2^-26 turns (2^-23.3 radians), sine and cosine to 2 ulp, three fp32 operations; the result to bf16
+    small = (a.abs() + b.abs()) * abs(amplitude) * 2.0 ** -20
+    tol[..., first] = tol[..., second] = small
+    return y, torch.where(tol > 0, tol * 1.01 + y.abs() * BF, 0.0)
+
+
+@pytest.mark.parametrize("layout", ("half", "interleaved"))
+@pytest.mark.parametrize("tokens,heads,kv_heads,dim,rotary", ((1, 16, 8, 128, 128), (3, 12, 12, 128, 64), (257, 6, 2, 96, 96), (1000, 4, 4, 80, 40), (37, 1, 1, 64, 2),
+                                                              (5, 2, 1, 36, 20), (64, 3, 3, 7, 6), (19, 128, 1, 64, 64), (2, 2, 2, 512, 256), (700, 32, 8, 128, 32)))
+def test_rotary(layout, tokens, heads, kv_heads, dim, rotary):
+    from sacq_b200 import rotary_frequencies, rotate_heads
+    gen = _gen(tokens)
+    q, k = _randn(gen, tokens, heads, dim), _randn(gen, tokens, kv_heads, dim)
+    freq, _ = rotary_frequencies(rotary)
+    for dtype, most, amplitude in ((torch.int32, 4096, 1.0), (torch.int64, 2 ** 33, 1.25)):
+        pos = torch.randint(0, most, (tokens,), generator=gen, device="cuda", dtype=dtype)
+        pos[0] = -3
+        for got, x in zip(rotate_heads(q, k, pos, freq, layout=layout, amplitude=amplitude), (q, k)):
+            ref, tol = _rotary_reference(x, pos, freq, layout, amplitude)
+            assert got.dtype == torch.bfloat16 and float(((got.double() - ref).abs() - tol).max()) <= 0
+
+
+@pytest.mark.parametrize("layout", ("half", "interleaved"))
+def test_rotary_views_and_in_place(layout):
+    from sacq_b200 import rotary_frequencies, rotate_heads
+    gen = _gen(1)
+    t, d = 300, 128
+    fused = _randn(gen, t, 6 * d)
+    freq, amp = rotary_frequencies(96, scaling={"kind": "yarn", "factor": 8.0, "original": 4096})
+    pos = torch.arange(t, device="cuda", dtype=torch.int32) + 70000
+    heads = [fused[:, :4 * d].view(t, 4, d), fused[:, 4 * d:5 * d].view(t, 1, d)]
+    refs = [_rotary_reference(x, pos, freq, layout, amp) for x in heads]
+    fresh = rotate_heads(*heads, pos, freq, layout=layout, amplitude=amp)
+    v = fused[:, 5 * d:].clone()
+    assert rotate_heads(*heads, pos, freq, layout=layout, amplitude=amp, out=tuple(heads))[0].data_ptr() == fused.data_ptr()
+    for x, f, (ref, tol) in zip(heads, fresh, refs):
+        assert torch.equal(x, f) and float(((x.double() - ref).abs() - tol).max()) <= 0
+    assert torch.equal(v, fused[:, 5 * d:])
+    # odd strides take the kernel for single elements; an inner stride and no key heads
+    odd = torch.nn.functional.pad(fresh[0], (0, 1))[..., :d]
+    again = rotate_heads(odd, None, pos, freq, layout=layout)
+    ref, tol = _rotary_reference(fresh[0], pos, freq, layout, 1.0)
+    assert again[1] is None and float(((again[0].double() - ref).abs() - tol).max()) <= 0
+    flipped = fresh[0].transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(rotate_heads(flipped, None, pos, freq, layout=layout)[0],
+                       rotate_heads(fresh[0], None, pos, freq, layout=layout)[0])
+    empty = rotate_heads(fresh[0][:0], fresh[1][:0], pos[:0], freq)
+    assert empty[0].shape == (0, 4, d) and empty[1].shape == (0, 1, d)
+
+
+# ----------------------------------------------------------------------------- norms around a block
+
+def _norm_reference(branch, residual, p, norm, post, eps, scale):
+    """(r, h, bound of r, bound of h) in float64; p: the vectors, as rows."""
+    one = lambda n, x: x if p[n] is None else p[n].double()  # noqa: E731
+    k = branch.shape[1]
+
+    def normed(x, kind, w, b, off):
+        """norm(x) w + b, and its error for an error `off` of x."""
+        c = x - x.mean(1, keepdim=True) if kind == "layer" else x
+        rstd = (c.square().mean(1, keepdim=True) + eps).rsqrt()
+        y = c * rstd * w
+        # the mean: k terms, and its share of off; the mean square: k terms, half of it on rstd, and the share of off on it
+        shift = k * F32 * x.abs().mean(1, keepdim=True) + off.mean(1, keepdim=True) if kind == "layer" else 0.0
+        each = off + shift
+        rel = (k / 2 + 10) * F32 + each.square().mean(1, keepdim=True).sqrt() * rstd
+        return y + b, (each * rstd * w).abs() + y.abs() * rel + (y.abs() + b.abs() if torch.is_tensor(b) else y.abs()) * 2 * F32
+
+    zero = torch.zeros(1, dtype=torch.float64, device=branch.device)
+    x, off = branch.double(), torch.zeros_like(branch, dtype=torch.float64)
+    if post:
+        x, off = normed(x, post, one("post_weight", zero + 1), one("post_bias", zero), off)
+    g = one("gate", zero + 1)
+    r = scale * residual.double() + g * x
+    off_r = (g * off).abs() + 3 * F32 * ((scale * residual.double()).abs() + (g * x).abs())
+    h, off_h = normed(r, norm, one("weight", zero + 1), one("bias", zero), off_r)
+    if p["mod_scale"] is not None:
+        m = 1 + p["mod_scale"].double()
+        off_h = (off_h * m).abs() + 4 * F32 * ((h * m).abs() + p["mod_shift"].double().abs())
+        h = h * m + p["mod_shift"].double()
+    return r, h, off_r * 1.01 + r.abs() * BF, off_h * 1.01
+
+
+def _norm_case(m, k, norm, post, vectors, seed, gated=True, modulated=True, affine=True, scale=1.0, by=1.0):
+    gen = _gen(seed)
+    branch, residual = _randn(gen, m, k, by=0.7 * by), _randn(gen, m, k, at=0.5 * by, by=by)
+    shape = (k,) if vectors == 0 else (vectors, k)
+    p = {"weight": _randn(gen, k, at=1.0, by=0.1) if affine else None, "bias": _randn(gen, k, by=0.1) if affine and norm == "layer" else None,
+         "post_weight": _randn(gen, k, at=1.0, by=0.1) if post and affine else None,
+         "post_bias": _randn(gen, k, by=0.1) if post == "layer" and affine else None,
+         "gate": _randn(gen, *shape, by=0.5) if gated else None, "mod_scale": _randn(gen, *shape, by=0.2) if modulated else None,
+         "mod_shift": _randn(gen, *shape, by=0.2) if modulated else None}
+    rows = torch.randint(0, vectors, (m,), generator=gen, device="cuda", dtype=torch.int32) if vectors and (gated or modulated) else None
+    each = {n: t if t is None or rows is None or n not in ("gate", "mod_scale", "mod_shift") else t[rows.long()] for n, t in p.items()}
+    return branch, residual, p, rows, _norm_reference(branch, residual, each, norm, post, 1e-6, scale)
+
+
+def _check_norm(got, ref, quantized=True):
+    r, h, tol_r, tol_h = ref
+    assert got[0].dtype == torch.bfloat16 and float(((got[0].double() - r).abs() - tol_r).max()) <= 0
+    if not quantized:
+        assert float(((got[1].double() - h).abs() - tol_h - h.abs() * BF * 1.01).max()) <= 0
+        return
+    q, s = got[1], got[2]
+    assert q.dtype == torch.float8_e4m3fn and s.dtype == torch.float32 and s.shape == (r.shape[0], 1)
+    top = h.abs().amax(1, keepdim=True)
+    want = torch.where(top > 0, top / 448, torch.ones_like(top))
+    off = tol_h.amax(1, keepdim=True) / 448 + want * 2 * F32
+    assert float(((s.double() - want).abs() - off).max()) <= 0
+    # e4m3: 2^-4 of the value, 2^-10 among the subnormal ones; the quotient and its saturation as exact as h and the scale
+    exact = h / s.double()
+    tol = exact.abs() * 2.0 ** -4 + 2.0 ** -10 + tol_h / s.double() * 1.1 + 448 * 4 * F32
+    assert float(((q.double() - exact).abs() - tol).max()) <= 0
+    if len(got) == 4:
+        assert float(((got[3].double() - h).abs() - tol_h - h.abs() * BF * 1.01).max()) <= 0
+
+
+@pytest.mark.parametrize("m,k", ((1, 1), (1, 8), (3, 7), (16, 1536), (2, 2048), (5, 1111), (130, 256), (1030, 264), (1500, 2048), (1025, 2047), (40, 6144),
+                                 (1100, 4096), (3, 8200), (2, 20000), (1, 32768)))
+@pytest.mark.parametrize("norm,post", (("rms", None), ("layer", "layer"), ("rms", "rms"), ("layer", None)))
+def test_residual_norm(m, k, norm, post):
+    from sacq_b200 import residual_norm_quantize_rows
+    branch, residual, p, rows, ref = _norm_case(m, k, norm, post, 0, seed=m + k)
+    got = residual_norm_quantize_rows(branch, residual, p["weight"], p["bias"], norm=norm, post_norm=post, post_weight=p["post_weight"],
+                                      post_bias=p["post_bias"], gate=p["gate"], mod_scale=p["mod_scale"], mod_shift=p["mod_shift"],
+                                      return_normalized=True)
+    _check_norm(got, ref)
+    plain = residual_norm_quantize_rows(branch, residual, p["weight"], p["bias"], norm=norm, post_norm=post, post_weight=p["post_weight"],
+                                        post_bias=p["post_bias"], gate=p["gate"], mod_scale=p["mod_scale"], mod_shift=p["mod_shift"],
+                                        quantize=False)
+    assert len(plain) == 2 and torch.equal(plain[0], got[0]) and torch.equal(plain[1], got[3])
+
+
+@pytest.mark.parametrize("m", (1, 19, 2100))
+def test_residual_norm_vectors_of_each_request(m):
+    from sacq_b200 import residual_norm_quantize_rows
+    for gated, modulated in ((True, False), (False, True), (True, True)):
+        branch, residual, p, rows, ref = _norm_case(m, 520, "layer", "rms", 5, seed=m, gated=gated, modulated=modulated, scale=0.75)
+        got = residual_norm_quantize_rows(branch, residual, p["weight"], p["bias"], norm="layer", post_norm="rms", post_weight=p["post_weight"],
+                                          gate=p["gate"], mod_scale=p["mod_scale"], mod_shift=p["mod_shift"], vector_rows=rows, residual_scale=0.75)
+        _check_norm(got, ref)
+    # a row outside of the table makes its own token NaN and no other
+    rows[0], keep = 5, residual_norm_quantize_rows(branch, residual, gate=p["gate"], vector_rows=rows, quantize=False)
+    bad = rows.clone()
+    bad[m // 2] = -1
+    got = residual_norm_quantize_rows(branch, residual, gate=p["gate"], vector_rows=bad, quantize=False)
+    clean = torch.ones(m, dtype=torch.bool, device="cuda")
+    clean[0] = clean[m // 2] = False
+    assert torch.equal(got[0][clean], keep[0][clean]) and bool(got[0][~clean].isnan().all()) and bool(got[1][~clean].isnan().all())
+
+
+def test_residual_norm_without_vectors_zeros_and_what_is_not_finite():
+    from sacq_b200 import residual_norm_quantize_rows
+    for m in (4, 1200):
+        branch, residual, p, rows, ref = _norm_case(m, 512, "rms", None, 0, seed=m, gated=False, modulated=False, affine=False, scale=0.5, by=30.0)
+        _check_norm(residual_norm_quantize_rows(branch, residual, residual_scale=0.5), ref)
+        branch[1], residual[1] = 0, 0
+        branch[2, 7], residual[3, 9] = INF, NAN
+        r, q, s = residual_norm_quantize_rows(branch, residual)
+        assert float(s[1]) == 1.0 and bool((q[1].float() == 0).all()) and bool((r[1] == 0).all())
+        assert bool(q[3].float().isnan().all()) and float(s[3]) == 1.0
+        assert bool(torch.isfinite(q[4:].float()).all()) and bool(q[2, 7].float().isnan())
+
+
+def test_residual_norm_reads_views_where_they_lie():
+    from sacq_b200 import residual_norm_quantize_rows
+    gen = _gen(2)
+    for m, k, pad in ((33, 512, 8), (1500, 512, 8), (33, 511, 1), (1500, 512, 3)):
+        both = _randn(gen, m, 2 * (k + pad))
+        branch, residual = both[:, :k], both[:, k + pad:2 * k + pad]
+        got = residual_norm_quantize_rows(branch, residual)
+        want = residual_norm_quantize_rows(branch.contiguous(), residual.contiguous())
+        if pad != 3:                                  # rows that are 16-byte aligned in one of the two only are summed in another order
+            assert _same(got, want)
+        _check_norm(got, _norm_reference(branch, residual, dict.fromkeys(("weight", "bias", "post_weight", "post_bias", "gate", "mod_scale", "mod_shift")),
+                                         "rms", None, 1e-6, 1.0))
+        across = residual.t().contiguous().t()
+        _check_norm(residual_norm_quantize_rows(branch, across), _norm_reference(branch, residual, dict.fromkeys(
+            ("weight", "bias", "post_weight", "post_bias", "gate", "mod_scale", "mod_shift")), "rms", None, 1e-6, 1.0))
+
+
+# ----------------------------------------------------------------------------- streams and graphs
+
+def _steps(x, inputs):
+    """A run of the operators together: norm, rotary, attention, norm."""
+    from sacq_b200 import attention_packed, residual_norm_quantize_rows, rotate_heads
+    r, h = residual_norm_quantize_rows(x, inputs["residual"], inputs["weight"], quantize=False)
+    t = h.view(x.shape[0], 8, 64)
+    q, k = rotate_heads(t[:, :4], t[:, 4:6], inputs["positions"], inputs["freq"])
+    a = attention_packed(q, k, t[:, 6:], inputs["cu"], causal=True)
+    return residual_norm_quantize_rows(torch.cat([a.reshape(x.shape[0], 256)] * 2, 1), r, gate=inputs["weight"], return_normalized=True)
+
+
+def _steps_inputs(seed, lengths):
+    from sacq_b200 import rotary_frequencies
+    gen = _gen(seed)
+    t = sum(lengths)
+    return _randn(gen, t, 512), {"residual": _randn(gen, t, 512), "weight": _randn(gen, 512, at=1.0, by=0.1), "cu": _offsets(lengths),
+                                 "positions": torch.cat([torch.arange(n) for n in lengths]).to(torch.int32).cuda(),
+                                 "freq": rotary_frequencies(64)[0]}
+
+
+def _same(a, b):
+    return all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b))
+
+
+def test_steps_together_and_in_graphs():
+    x, inputs = _steps_inputs(1, [200, 30, 1, 90])
+    want = _steps(x, inputs)
+    # the steps one by one in float64, from each step's own bf16 inputs
+    from sacq_b200 import attention_packed, residual_norm_quantize_rows, rotate_heads
+    none = dict.fromkeys(("weight", "bias", "post_weight", "post_bias", "gate", "mod_scale", "mod_shift"))
+    r, h = residual_norm_quantize_rows(x, inputs["residual"], inputs["weight"], quantize=False)
+    _check_norm((r, h), _norm_reference(x, inputs["residual"], {**none, "weight": inputs["weight"]}, "rms", None, 1e-6, 1.0), False)
+    t = h.view(-1, 8, 64)
+    q, k = rotate_heads(t[:, :4], t[:, 4:6], inputs["positions"], inputs["freq"])
+    a, lse = attention_packed(q, k, t[:, 6:], inputs["cu"], causal=True, return_lse=True)
+    lengths = [200, 30, 1, 90]
+    _check_attention(a, lse, _attention_reference(q, k, t[:, 6:], lengths, lengths, True))
+    branch = torch.cat([a.reshape(-1, 256)] * 2, 1)
+    _check_norm(want, _norm_reference(branch, r, {**none, "gate": inputs["weight"]}, "rms", None, 1e-6, 1.0))
+    # two graphs of the same calls, replayed on streams of their own, with other inputs copied in
+    graphs = []
+    for seed in (2, 3):
+        xs, ins = _steps_inputs(seed, [200, 30, 1, 90])
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            _steps(xs, ins)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            made = _steps(xs, ins)
+        graphs.append((g, xs, ins, made))
+    other = [_steps_inputs(seed, [200, 30, 1, 90]) for seed in (4, 5)]
+    wants = [_steps(*o) for o in other]
+    for (g, xs, ins, made), (nx, nins) in zip(graphs, other):
+        xs.copy_(nx)
+        ins["residual"].copy_(nins["residual"])
+        ins["weight"].copy_(nins["weight"])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(3):
+        for s, (g, *_rest) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(_same(made, w) for (_, _, _, made), w in zip(graphs, wants))
+
+
+def test_attention_split_over_keys_in_graphs_on_two_streams():
+    """A long past is worked on in parts whose results are joined: each call has its own room for them."""
+    from sacq_b200 import attention_packed
+    sets = []
+    for seed in range(4):
+        gen = _gen(seed)
+        q, k, v = _randn(gen, 2, 4, 128), _randn(gen, 9000, 2, 128), _randn(gen, 9000, 2, 128)
+        sets.append((q, k, v, _offsets([1, 1]), _offsets([7000, 2000])))
+    want = [attention_packed(*s, causal=True) for s in sets]
+    for s, w in zip(sets, want):
+        ref = _attention_reference(*s[:3], [1, 1], [7000, 2000], True)
+        assert float(((w.double() - ref[0]).abs() - ref[2]).max()) <= 0
+    streams = [torch.cuda.Stream() for _ in sets]
+    graphs, outs = [], []
+    for s in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(attention_packed(*s, causal=True))
+        graphs.append(g)
+    for _ in range(5):
+        for st, g in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+        eager = []
+        for st, s in zip(streams, sets):
+            with torch.cuda.stream(st):
+                eager.append(attention_packed(*s, causal=True))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, w) for a, w in zip(outs, want)) and all(torch.equal(a, w) for a, w in zip(eager, want))
+
+
+def test_steps_follow_the_kernel_in_front():
+    """Each step is launched early behind its predecessor and reads nothing before that one has finished."""
+    x, inputs = _steps_inputs(6, [150, 90])
+    want = _steps(x.clone() * 0.5, inputs)
+    big = torch.randn(4096, 4096, device="cuda")
+    for _ in range(3):
+        y = x * 0
+        for _ in range(3):
+            big = big @ big * 1e-3
+        y.add_(x, alpha=0.5)
+        assert _same(_steps(y, inputs), want)
