@@ -63,6 +63,12 @@ __device__ void attend_row(const AttnParams& p, const uint16_t* q, const uint16_
   }
 }
 
-int launch_attention_rows(const AttnParams& p, cudaStream_t s);
+int launch_attention_rows(const AttnParams& p, cudaStream_t s);          // any head dim up to 256, any alignment
+
+// Tensor cores: head dims that are multiples of 8 up to 128, rows that TMA can read.
+bool attention_tmem_supported(const AttnParams& p);
+int64_t attention_tmem_workspace(const AttnParams& p);
+int attention_tmem_status(int* out);
+int launch_attention_tmem(const AttnParams& p, void* workspace, int64_t workspace_bytes, cudaStream_t s);
 
 }  // namespace sacq

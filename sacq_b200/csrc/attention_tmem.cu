@@ -1,0 +1,873 @@
+// Attention over packed sequences on the tensor cores (sm_100a), head dims up to 128, persistent CTAs.
+//
+// A tile is 128 rows of queries: 128 / pack tokens x `pack` heads of one key-value head (pack: the largest power of two
+// that divides the group), so that single tokens share a tile with the other heads of their group and a causal tile's
+// diagonal is 128 / pack keys wide.  Keys come 128 at a time:
+//   S = Q K^T        tcgen05.mma, Q and K tiles in shared memory (TMA, SWIZZLE_128B), S in tensor memory, fp32
+//   P = exp(S - m)   one thread per row: running maximum and sum, no shuffles; P goes back over S as bf16
+//   O += P V         tcgen05.mma with P from tensor memory as A, the V tile as it lies (MN-major B), O in tensor memory
+// P is rounded to bf16 because V is bf16 and one instruction's operands have one type; its sum is taken before that.
+// O is rescaled only when a row's maximum has risen by more than 2^8 since the last time: until then exp(S - m) stays
+// below 256, which bf16 and the fp32 sums hold as exactly as values below 1.
+//
+// An item of work is a pair of tiles of one sequence and head group, over its keys or a chunk of them.  Both tiles
+// share the K and V tiles, each has its warpgroup, S and O: while the tensor cores work for one, the other's
+// exponentials are taken.  Where the sequence has one tile's tokens only, the two warpgroups take its keys in turn and their
+// results are joined.  Chunks (few items, many keys) leave fp32 results, joined by a second kernel in a fixed order.
+//
+// Roles: warps 0-3 and 4-7 softmax and epilogue of the two tiles, warp 8 MMA issuer and TMEM owner, warp 9 TMA and the
+// list of items.  Every mbarrier wait is bounded (status word + CTA-wide abort flag).
+#include <cuda.h>
+
+#include "attention.cuh"
+#include "umma.cuh"
+
+namespace sacq {
+
+namespace {
+
+using namespace umma;
+
+constexpr int kTile = 128;
+constexpr int kThreads = 320;
+constexpr int kMmaWarp = 8, kLoadWarp = 9;
+constexpr float kRescale = 8.0f;            // log2
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ int g_status;                    // nonzero: a wait ran out
+
+struct TmemAttnParams {
+  AttnParams a;
+  int pack_log2;                            // heads of a tile
+  int groups;                               // heads / pack
+  int chunk;                                // key tiles of a chunk
+  int chunks_most;                          // chunks of the longest sequence possible; 1: results go straight to out
+  float* part_o;                            // [chunks_most][tokens_q][heads][dim]
+  float* part_lse;                          // [chunks_most][tokens_q][heads]
+};
+
+struct Item {
+  int last;                                 // no more items
+  int q_row, q_left;                        // first query row; rows of the sequence from it on
+  int head, kv_head;
+  int k_row, keys;                          // first key row, keys of the chunk
+  int base;                                 // causal: token t of the item sees min(keys, base + t + 1), else keys
+  int n, n0;                                // key tiles of the item (dual: of the second tile), dual: of the first
+  int dual;
+  int part;                                 // chunk, or -1: the whole result
+};
+
+template <int DP>
+struct Shape {
+  static constexpr int kHalves = DP / 64;
+  static constexpr int kTileBytes = kTile * DP * 2;
+  static constexpr int kHalfBytes = kTile * 128;          // 64 bf16 of every row
+  static constexpr int kStages = DP == 128 ? 4 : 8;
+  static constexpr uint32_t kQ = 0;
+  static constexpr uint32_t kRing = 2 * kTileBytes;
+  static constexpr uint32_t kJoin = kRing + kStages * kTileBytes;   // 128 rows x 64 fp32
+  static constexpr uint32_t kJoinMl = kJoin + kTile * 256;          // 128 x (m, l)
+  static constexpr uint32_t kBars = kJoinMl + kTile * 8;
+  static constexpr uint32_t kItems = kBars + 8 * 64;
+  static constexpr uint32_t kMisc = kItems + 2 * 64;
+  static constexpr uint32_t kTotal = kMisc + 64;
+  // tensor memory columns
+  static constexpr int kS = 0, kO = 256;
+};
+// mbarriers
+constexpr int Q_FULL = 0, Q_EMPTY = 1, S_FULL = 2, P_FULL = 4, O_FULL = 6, ITEM_FULL = 8, ITEM_EMPTY = 10, DRAIN = 12,
+              KV_FULL = 16, KV_EMPTY = 32, JOIN_FULL = 48, JOIN_EMPTY = 52;
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void umma_bf16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_bf16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// fp32 accumulator, bf16 operands, A K-major, B K-major or (b_mn) MN-major, M = 128.
+__device__ __forceinline__ uint32_t idesc_bf16(int n, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+}
+// MN-major operand (a V tile): 64 columns x 8 rows to a swizzle atom, 1024 bytes from one group of 8 rows to the next, `half`
+// bytes from 64 columns to the next 64.
+__device__ __forceinline__ uint64_t make_mn_desc(uint32_t addr, uint32_t half) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr & 0x3FFFF) >> 4);
+  d |= (uint64_t)(half >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {      // without waiting
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// Waits for the loads of this thread; the registers pass through, so that no use of them moves in front of it.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :: "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Keys that token t of an item sees.
+__device__ __forceinline__ int seen(const Item& it, bool causal, int t) { return causal ? max(0, min(it.keys, it.base + t + 1)) : it.keys; }
+__device__ __forceinline__ int key_tiles(int keys) { return (keys + kTile - 1) / kTile; }
+// Columns of key tile j that the tile's last token sees, in whole instructions of 16.
+__device__ __forceinline__ int columns(int most, int j) { return (min(kTile, most - j * kTile) + 15) & ~15; }
+
+// One output row by a warp, for rows that a non-finite value of a key they do not see got into (0 x inf): the keys that they
+// see, one after another.
+__device__ __noinline__ void redo_row(const TmemAttnParams& p, const Item& it, int64_t token, int head, int keys) {
+  const AttnParams& a = p.a;
+  const int lane = threadIdx.x & 31;
+  RowState<4> st;
+  attend_row<4>(a, a.q + token * a.q_token + head * a.q_head, a.k + it.k_row * a.k_token + it.kv_head * a.k_head,
+                a.v + it.k_row * a.v_token + it.kv_head * a.v_head, keys, st);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int d = lane + 32 * e;
+    if (d >= a.dim) continue;
+    const float o = st.acc[e] / st.l;
+    if (it.part < 0) a.out[token * a.out_token + head * a.out_head + d] = float_to_bf16_bits(o);
+    else p.part_o[(((int64_t)it.part * a.tokens_q + token) * a.heads + head) * a.dim + d] = o;
+  }
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TmemAttnParams p) {
+  using Sh = Shape<DP>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t sm = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const sp = smem_raw + (sm - smem_u32(smem_raw));
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(sp + Sh::kMisc);
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(sp + Sh::kMisc + 8);
+  Item* const items = reinterpret_cast<Item*>(sp + Sh::kItems);       // two of 64 bytes
+  auto item_at = [&](uint32_t i) { return reinterpret_cast<Item*>(reinterpret_cast<uint8_t*>(items) + (i & 1) * 64); };
+  auto bar = [&](int i) { return sm + Sh::kBars + 8u * i; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const AttnParams& a = p.a;
+  const int tokens_log2 = 7 - p.pack_log2;                              // tokens of a tile
+  const int tile_tokens = 1 << tokens_log2;
+  const bool causal = a.causal != 0;
+  static_assert(sizeof(Item) <= 64, "item slots");
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) {
+    mbar_init(bar(Q_FULL), 1);
+    mbar_init(bar(Q_EMPTY), 1);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(bar(S_FULL + w), 1);
+      mbar_init(bar(P_FULL + w), 4);
+      mbar_init(bar(O_FULL + w), 1);
+      mbar_init(bar(ITEM_FULL + w), 1);
+      mbar_init(bar(ITEM_EMPTY + w), 9);
+    }
+    mbar_init(bar(DRAIN), 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(bar(JOIN_FULL + i), 1);
+      mbar_init(bar(JOIN_EMPTY + i), 1);
+    }
+    for (int s = 0; s < Sh::kStages; ++s) {
+      mbar_init(bar(KV_FULL + s), 1);
+      mbar_init(bar(KV_EMPTY + s), 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async();
+  }
+  if (warp == kMmaWarp) tmem_alloc(smem_u32(tmem_slot), 512);
+  if (warp == kLoadWarp && lane == 0) {
+    prefetch_tensormap(&map_q);
+    prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  if (warp == kLoadWarp) {
+    // ---- the list of items, and the copies they need
+    uint32_t c = 0, nq = 0, made = 0;        // key / value tiles, items with keys, items so far
+    bool ok = true;
+    auto take = [&](const CUtensorMap* map, const Item& it, int j) {
+      const uint32_t s = c % Sh::kStages;
+      ok = ok && mbar_wait_warp(bar(KV_EMPTY + s), ((c / Sh::kStages) & 1) ^ 1, abort_flag, &g_status);
+      if (!ok) return;
+      if (elect_one()) {
+        mbar_arrive_expect_tx(bar(KV_FULL + s), Sh::kTileBytes);
+        for (int h = 0; h < Sh::kHalves; ++h)
+          tma_load_3d(sm + Sh::kRing + s * Sh::kTileBytes + h * Sh::kHalfBytes, map, h * 64, it.kv_head, it.k_row + j * kTile, bar(KV_FULL + s));
+      }
+      __syncwarp();
+      ++c;
+    };
+    // sequences are looked at 32 at a time: this lane's number of items and the items in front of it
+    int window = 0;
+    int64_t before = 0;                      // items of the sequences in front of the window
+    int64_t mine = 0, upto = 0;
+    Span sq = {0, 0}, sk = {0, 0};
+    int chunks = 1;
+    auto look = [&] {
+      const int s = window + lane;
+      mine = 0;
+      sq = sk = {0, 0};
+      chunks = 1;
+      if (s < a.sequences) {
+        sq = span_of(a.cu_q, s, a.tokens_q);
+        sk = span_of(a.cu_k, s, a.tokens_k);
+        const int64_t pairs = (sq.length + 2 * tile_tokens - 1) >> (tokens_log2 + 1);
+        if (p.chunks_most > 1) chunks = max(1, (int)((key_tiles((int)sk.length) + p.chunk - 1) / p.chunk));
+        mine = pairs * chunks * p.groups;
+      }
+      upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+    };
+    look();
+    for (int64_t index = blockIdx.x; ok; index += gridDim.x) {
+      while (window < a.sequences && index >= before + __shfl_sync(0xffffffffu, upto, 31)) {
+        before += __shfl_sync(0xffffffffu, upto, 31);
+        window += 32;
+        look();
+      }
+      const uint32_t found = __ballot_sync(0xffffffffu, index < before + upto);
+      Item it = {};
+      it.last = window >= a.sequences || found == 0;
+      if (!it.last) {
+        const int src = __ffs(found) - 1;
+        const int64_t sq_begin = __shfl_sync(0xffffffffu, sq.begin, src), lq = __shfl_sync(0xffffffffu, sq.length, src);
+        const int64_t sk_begin = __shfl_sync(0xffffffffu, sk.begin, src), lk = __shfl_sync(0xffffffffu, sk.length, src);
+        const int nchunks = __shfl_sync(0xffffffffu, chunks, src);
+        const int64_t start = before + __shfl_sync(0xffffffffu, upto, src) - __shfl_sync(0xffffffffu, mine, src);
+        // heads first, then chunks; the pairs of tiles from the last, longest one to the first
+        int64_t r = index - start;
+        const int pairs = (int)((lq + 2 * tile_tokens - 1) >> (tokens_log2 + 1));
+        const int group = (int)(r % p.groups);
+        r /= p.groups;
+        const int part = (int)(r % nchunks);
+        const int pair = pairs - 1 - (int)(r / nchunks);
+        const int t0 = pair * 2 * tile_tokens;
+        const int tiles = key_tiles((int)lk);
+        const int first = part * p.chunk, n = nchunks > 1 ? min(p.chunk, tiles - first) : tiles;
+        it.q_row = (int)(sq_begin + t0);
+        it.q_left = (int)lq - t0;
+        it.head = group << p.pack_log2;
+        it.kv_head = it.head / (a.heads / a.kv_heads);
+        it.k_row = (int)sk_begin + (nchunks > 1 ? first * kTile : 0);
+        it.keys = nchunks > 1 ? min((int)lk - first * kTile, n * kTile) : (int)lk;
+        it.base = (int)(lk - lq) + t0 - (nchunks > 1 ? first * kTile : 0);
+        it.dual = it.q_left > tile_tokens;
+        const int most = seen(it, causal, min(it.q_left, it.dual ? 2 * tile_tokens : tile_tokens) - 1);
+        it.n = key_tiles(most);
+        it.n0 = it.dual ? key_tiles(seen(it, causal, tile_tokens - 1)) : 0;
+        it.part = nchunks > 1 ? part : -1;
+      }
+      ok = mbar_wait_warp(bar(ITEM_EMPTY + (made & 1)), ((made >> 1) & 1) ^ 1, abort_flag, &g_status);
+      if (!ok) break;
+      if (lane == 0) {
+        *item_at(made) = it;
+        mbar_arrive(bar(ITEM_FULL + (made & 1)));
+      }
+      __syncwarp();
+      ++made;
+      if (it.last) break;
+      if (it.n == 0) continue;
+      ok = mbar_wait_warp(bar(Q_EMPTY), (nq & 1) ^ 1, abort_flag, &g_status);
+      if (!ok) break;
+      ++nq;
+      if (elect_one()) {
+        mbar_arrive_expect_tx(bar(Q_FULL), (it.dual ? 2 : 1) * Sh::kTileBytes);
+        for (int w = 0; w < (it.dual ? 2 : 1); ++w)
+          for (int h = 0; h < Sh::kHalves; ++h)
+            tma_load_3d(sm + Sh::kQ + w * Sh::kTileBytes + h * Sh::kHalfBytes, &map_q, h * 64, it.head, it.q_row + w * tile_tokens, bar(Q_FULL));
+      }
+      __syncwarp();
+      // in the order of their use: K of the first step (one tile: of two), then V of a step and K of the next (next but one)
+      const int ahead = it.dual ? 1 : 2;
+      for (int j = 0; j < min(ahead, it.n); ++j) take(&map_k, it, j);
+      for (int j = 0; j < it.n; ++j) {
+        take(&map_v, it, j);
+        if (j + ahead < it.n) take(&map_k, it, j + ahead);
+      }
+    }
+    if (*abort_flag)                         // copies in flight land before the CTA leaves
+      for (uint32_t i = c > Sh::kStages ? c - Sh::kStages : 0; i < c; ++i)
+        for (int t = 0; t < 100000 && !mbar_try_wait(bar(KV_FULL + i % Sh::kStages), (i / Sh::kStages) & 1); ++t) {}
+  } else if (warp == kMmaWarp) {
+    // ---- MMA issuer
+    uint32_t c = 0, nq = 0, np[2] = {0, 0};
+    const int k_steps = (a.dim + 15) / 16;
+    const uint32_t pv_n = (uint32_t)k_steps * 16;
+    const uint32_t idesc_pv = idesc_bf16((int)pv_n, true);
+    bool ok = true;
+    auto next = [&]() -> uint32_t {          // the next tile of the ring
+      const uint32_t s = c % Sh::kStages;
+      ok = ok && mbar_wait_warp(bar(KV_FULL + s), (c / Sh::kStages) & 1, abort_flag, &g_status);
+      ++c;
+      return s;
+    };
+    auto commit = [&](int b) {
+      if (elect_one()) umma_commit(bar(b));
+      __syncwarp();
+    };
+    auto qk = [&](int w, int tile, uint32_t s, int n) {       // S of warpgroup w from Q tile `tile`
+      if (!ok) return;
+      const uint32_t idesc = warp_uniform(idesc_bf16(n, false));
+      const uint32_t q0 = sm + Sh::kQ + tile * Sh::kTileBytes, k0 = sm + Sh::kRing + s * Sh::kTileBytes;
+      if (elect_one()) {
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          const uint32_t off = (i >> 2) * Sh::kHalfBytes + (i & 3) * 32;
+          if (i < k_steps) umma_bf16_ss(tmem + Sh::kS + w * kTile, make_smem_desc(q0 + off), make_smem_desc(k0 + off), idesc, i > 0);
+        }
+      }
+      __syncwarp();
+    };
+    auto pv = [&](int w, uint32_t s, int n, bool first) {     // O of warpgroup w += P V over the tile's first n keys
+      ok = ok && mbar_wait_warp(bar(P_FULL + w), np[w] & 1, abort_flag, &g_status);
+      ++np[w];
+      if (!ok) return;
+      tc_fence_after();
+      const uint32_t v0 = sm + Sh::kRing + s * Sh::kTileBytes;
+      if (elect_one()) {
+#pragma unroll
+        for (int i = 0; i < kTile / 16; ++i)
+          if (i * 16 < n)
+            umma_bf16_ts(tmem + Sh::kO + w * DP, tmem + Sh::kS + w * kTile + i * 8, make_mn_desc(v0 + i * 2048, Sh::kHalfBytes), idesc_pv, !first || i > 0);
+      }
+      __syncwarp();
+    };
+    // rows of a V tile behind the last key, up to a whole instruction: zeros, whatever lies there in memory
+    auto clear_tail = [&](uint32_t s, int keys) {
+      if (!ok || keys >= kTile || (keys & 15) == 0) return;
+      const int end = (keys + 15) & ~15;
+      for (int i = lane; i < (end - keys) * 8 * Sh::kHalves; i += 32) {
+        const int row = keys + (i >> 3) / Sh::kHalves, h = (i >> 3) % Sh::kHalves;
+        *reinterpret_cast<uint4*>(sp + Sh::kRing + s * Sh::kTileBytes + h * Sh::kHalfBytes + row * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async();
+      __syncwarp();
+    };
+    for (uint32_t i = 0; ok; ++i) {
+      if (!mbar_wait_warp(bar(ITEM_FULL + (i & 1)), (i >> 1) & 1, abort_flag, &g_status)) break;
+      const Item it = *item_at(i);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(ITEM_EMPTY + (i & 1)));
+      if (it.last) break;
+      if (it.n == 0) continue;
+      if (!mbar_wait_warp(bar(Q_FULL), nq & 1, abort_flag, &g_status)) break;
+      ++nq;
+      const int most = seen(it, causal, min(it.q_left, it.dual ? 2 * tile_tokens : tile_tokens) - 1);
+      if (it.dual) {
+        const int most0 = seen(it, causal, tile_tokens - 1);
+        uint32_t ks = next();
+        if (it.n0 > 0) {
+          qk(0, 0, ks, columns(most0, 0));
+          commit(S_FULL + 0);
+        }
+        qk(1, 1, ks, columns(most, 0));
+        commit(S_FULL + 1);
+        commit(KV_EMPTY + ks);
+        if (it.n == 1) commit(Q_EMPTY);
+        for (int j = 0; j < it.n && ok; ++j) {
+          const uint32_t vs = next();
+          clear_tail(vs, it.keys - j * kTile);
+          if (j < it.n0) pv(0, vs, columns(most0, j), j == 0);
+          if (j + 1 < it.n) ks = next();
+          if (j + 1 < it.n0) {
+            qk(0, 0, ks, columns(most0, j + 1));
+            commit(S_FULL + 0);
+          } else if (j + 1 == it.n0) {
+            commit(O_FULL + 0);
+          }
+          pv(1, vs, columns(most, j), j == 0);
+          commit(KV_EMPTY + vs);
+          if (j + 1 < it.n) {
+            qk(1, 1, ks, columns(most, j + 1));
+            commit(S_FULL + 1);
+            commit(KV_EMPTY + ks);
+            if (j + 2 == it.n) commit(Q_EMPTY);
+          } else {
+            commit(O_FULL + 1);
+          }
+        }
+      } else {
+        for (int j = 0; j < min(2, it.n); ++j) {
+          const uint32_t ks = next();
+          qk(j, 0, ks, columns(most, j));
+          commit(S_FULL + j);
+          commit(KV_EMPTY + ks);
+        }
+        if (it.n <= 2) commit(Q_EMPTY);
+        for (int j = 0; j < it.n && ok; ++j) {
+          const int w = j & 1;
+          const uint32_t vs = next();
+          clear_tail(vs, it.keys - j * kTile);
+          pv(w, vs, columns(most, j), j < 2);
+          commit(KV_EMPTY + vs);
+          if (j + 2 < it.n) {
+            const uint32_t ks = next();
+            qk(w, 0, ks, columns(most, j + 2));
+            commit(S_FULL + w);
+            commit(KV_EMPTY + ks);
+            if (j + 3 == it.n) commit(Q_EMPTY);
+          } else {
+            commit(O_FULL + w);
+          }
+        }
+      }
+    }
+    commit(DRAIN);                           // nothing of this CTA is in flight when it gives its tensor memory back
+    for (int t = 0; t < 1000000 && !mbar_try_wait(bar(DRAIN), 0); ++t) {}
+  } else {
+    // ---- softmax and epilogue: warpgroup w, one row per thread
+    const int w = warp >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_at = tmem + lanes + Sh::kS + w * kTile, o_at = tmem + lanes + Sh::kO + w * DP;
+    const float c2 = a.scale * kLog2e;
+    uint32_t ns = 0, no = 0, nj = 0;         // steps, items with keys, halves joined
+    float* const join = reinterpret_cast<float*>(sp + Sh::kJoin) + row * 64;
+    float* const join_ml = reinterpret_cast<float*>(sp + Sh::kJoinMl) + row * 2;
+    bool ok = true;
+    for (uint32_t i = 0; ok; ++i) {
+      if (!mbar_wait_warp(bar(ITEM_FULL + (i & 1)), (i >> 1) & 1, abort_flag, &g_status)) break;
+      const Item it = *item_at(i);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(ITEM_EMPTY + (i & 1)));
+      if (it.last) break;
+      const int t = (row >> p.pack_log2) + (it.dual ? w * tile_tokens : 0);      // token of the item
+      const bool valid = t < it.q_left;
+      const bool live = __any_sync(0xffffffffu, valid);
+      const int mine = valid ? seen(it, causal, t) : it.keys;
+      const int least = __reduce_min_sync(0xffffffffu, mine);
+      const int tiles = it.dual && w == 0 ? it.n0 : it.n, step = it.dual ? 1 : 2;
+      float m = -INFINITY, l = 0.f;          // m: the maximum that the weights are taken against
+      bool first = true;
+      for (int j = it.dual ? 0 : w; j < tiles; j += step) {
+        if (!mbar_wait_warp(bar(S_FULL + w), ns & 1, abort_flag, &g_status)) { ok = false; break; }
+        ++ns;
+        if (live) {
+          tc_fence_after();
+          uint32_t s[4][32];
+#pragma unroll
+          for (int b = 0; b < 4; ++b) tmem_ld32(s_at + b * 32, s[b]);
+#pragma unroll
+          for (int b = 0; b < 4; ++b) tmem_wait_ld(s[b]);
+          if ((j + 1) * kTile > least) {     // columns that this row does not see
+            const int end = mine - j * kTile;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (b * 32 + e >= end) s[b][e] = 0xff800000u;
+          }
+          float top[4];
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            top[b] = __uint_as_float(s[b][0]);
+#pragma unroll
+            for (int e = 1; e < 32; ++e) top[b] = fmaxf(top[b], __uint_as_float(s[b][e]));
+          }
+          const float high = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+          if (__any_sync(0xffffffffu, (high - m) * c2 > kRescale)) {
+            const float keep = m == -INFINITY ? 0.f : exp2_fast((m - high) * c2);
+            m = high;
+            l *= keep;
+            if (!first) {
+#pragma unroll 1
+              for (int b = 0; b < DP / 32; ++b) {
+                uint32_t o[32];
+                tmem_ld32(o_at + b * 32, o);
+                tmem_wait_ld(o);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                tmem_st32(o_at + b * 32, o);
+              }
+            }
+          }
+          const float base = m == -INFINITY ? 0.f : m * c2;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int b = 0; b < 4; b += 2) {
+            uint32_t w2[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float x = exp2_fast(fmaf(__uint_as_float(s[b + (e >> 4)][2 * (e & 15)]), c2, -base));
+              const float y = exp2_fast(fmaf(__uint_as_float(s[b + (e >> 4)][2 * (e & 15) + 1]), c2, -base));
+              sum[e & 3] += x + y;
+              w2[e] = bf16_pair(x, y);
+            }
+            tmem_st32(s_at + b * 16, w2);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_wait_st();
+          first = false;
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(P_FULL + w));
+      }
+      if (!ok) break;
+      const bool any = (it.dual ? 0 : w) < tiles;
+      if (any) {
+        if (!mbar_wait_warp(bar(O_FULL + w), no & 1, abort_flag, &g_status)) break;
+        ++no;
+        tc_fence_after();
+      }
+      if (!live) continue;
+      // one tile's keys were taken in turn: the second warpgroup hands over its sums, 64 columns at a time
+      const bool joined = !it.dual && it.n > 1;
+      if (!it.dual && w == 1) {
+        if (!joined) continue;
+#pragma unroll 1
+        for (int h = 0; h < Sh::kHalves && ok; ++h) {
+          uint32_t o[2][32];
+          tmem_ld32(o_at + h * 64, o[0]);
+          tmem_ld32(o_at + h * 64 + 32, o[1]);
+          tmem_wait_ld(o[0]);
+          tmem_wait_ld(o[1]);
+          ok = mbar_wait_warp(bar(JOIN_EMPTY + quarter), (nj & 1) ^ 1, abort_flag, &g_status);
+          if (!ok) break;
+          ++nj;
+          if (h == 0) *reinterpret_cast<float2*>(join_ml) = make_float2(m, l);
+          // 16-byte pieces, shifted by the row so that the lanes of a warp fall on different banks
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint32_t* u = &o[e >> 3][4 * (e & 7)];
+            *reinterpret_cast<uint4*>(join + ((e ^ (row & 15)) << 2)) = make_uint4(u[0], u[1], u[2], u[3]);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(JOIN_FULL + quarter));
+        }
+        continue;
+      }
+      const int64_t token = (int64_t)it.q_row + t;
+      const int head = it.head + (row & ((1 << p.pack_log2) - 1));
+      uint16_t* const out = a.out + token * a.out_token + head * a.out_head;
+      const int64_t slot = ((int64_t)max(it.part, 0) * a.tokens_q + token) * a.heads + head;
+      float inv = 0.f, scale0 = 1.f, scale1 = 0.f;
+      bool finite = true;
+#pragma unroll 1
+      for (int b = 0; b < DP / 32; ++b) {
+        uint32_t o[32];
+        if (any) {
+          tmem_ld32(o_at + b * 32, o);
+          tmem_wait_ld(o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        }
+        if (joined) {
+          if ((b & 1) == 0) {
+            ok = mbar_wait_warp(bar(JOIN_FULL + quarter), nj & 1, abort_flag, &g_status);
+            if (!ok) break;
+            ++nj;
+          }
+          if (b == 0) {
+            const float2 ml = *reinterpret_cast<const float2*>(join_ml);
+            const float high = fmaxf(m, ml.x);
+            scale0 = m == -INFINITY ? 0.f : exp2_fast((m - high) * c2);
+            scale1 = ml.x == -INFINITY ? 0.f : exp2_fast((ml.x - high) * c2);
+            l = l * scale0 + ml.y * scale1;
+            m = high;
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint4 v = *reinterpret_cast<const uint4*>(join + ((((b & 1) * 8 + e) ^ (row & 15)) << 2));
+            const uint32_t* u = &v.x;
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+              o[4 * e + f] = __float_as_uint(fmaf(__uint_as_float(u[f]), scale1, __uint_as_float(o[4 * e + f]) * scale0));
+          }
+          __syncwarp();
+          if ((b & 1) && lane == 0) mbar_arrive(bar(JOIN_EMPTY + quarter));
+        }
+        if (b == 0) inv = mine > 0 ? 1.0f / l : 0.f;
+        if (valid) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float x = mine > 0 ? __uint_as_float(o[e]) * inv : 0.f;
+            finite = finite && fabsf(x) < INFINITY;
+            o[e] = __float_as_uint(x);
+          }
+          if (it.part < 0) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float* f = reinterpret_cast<const float*>(&o[8 * e]);
+              if (b * 32 + e * 8 < a.dim)
+                *reinterpret_cast<uint4*>(out + b * 32 + e * 8) =
+                    make_uint4(bf16_pair(f[0], f[1]), bf16_pair(f[2], f[3]), bf16_pair(f[4], f[5]), bf16_pair(f[6], f[7]));
+            }
+          } else {
+            float* const po = p.part_o + slot * a.dim;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (b * 32 + e * 4 < a.dim) *reinterpret_cast<uint4*>(po + b * 32 + e * 4) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+        }
+        __syncwarp();
+      }
+      if (!ok) break;
+      if (valid) {
+        const float le = mine > 0 ? fmaf(m, a.scale, logf(l)) : -INFINITY;
+        if (it.part >= 0) p.part_lse[slot] = le;
+        else if (a.lse != nullptr) a.lse[token * a.heads + head] = le;
+      }
+      // a value that is not finite may have come in with a weight of zero: from keys that other rows of the tile see, or
+      // that share an instruction with them
+      const int most = seen(it, causal, min(it.q_left, (it.dual && w == 1 ? 2 : 1) * tile_tokens) - 1);
+      __syncwarp();                          // the rows as they are lie in front of the ones made again
+      uint32_t odd = __ballot_sync(0xffffffffu, valid && !finite && mine > 0 && mine < min((most + 15) & ~15, it.keys));
+      while (odd != 0) {
+        const int src = __ffs(odd) - 1;
+        odd &= odd - 1;
+        redo_row(p, it, __shfl_sync(0xffffffffu, token, src), __shfl_sync(0xffffffffu, head, src), __shfl_sync(0xffffffffu, mine, src));
+      }
+    }
+  }
+  // ---- common exit: every thread arrives here, also after an aborted wait
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+}
+
+// Joins the chunks of a query: a warp per row and head.
+__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ TmemAttnParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const AttnParams& a = p.a;
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int64_t token = item / a.heads;
+  const int head = (int)(item - token * a.heads);
+  if (token >= a.tokens_q) return;
+  int lo = 0, hi = a.sequences;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.cu_q[mid] <= token) lo = mid; else hi = mid;
+  }
+  const Span sq = span_of(a.cu_q, lo, a.tokens_q);
+  if (token < sq.begin || token >= sq.begin + sq.length) return;
+  const Span sk = span_of(a.cu_k, lo, a.tokens_k);
+  const int chunks = (key_tiles((int)sk.length) + p.chunk - 1) / p.chunk;
+  if (chunks <= 1) return;                   // written by the attention kernel
+  const int64_t stride = a.tokens_q * a.heads, at = token * a.heads + head;
+  float m = -INFINITY;
+  for (int i = lane; i < chunks; i += 32) m = fmaxf(m, p.part_lse[i * stride + at]);
+  m = warp_max(m);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+  const int d = lane * 4;
+  for (int i = 0; i < chunks; ++i) {
+    const float le = p.part_lse[i * stride + at];
+    if (le == -INFINITY) continue;
+    const float f = exp2f((le - base) * kLog2e);
+    l += f;
+    if (d < a.dim) {
+      const float4 v = *reinterpret_cast<const float4*>(p.part_o + (i * stride + at) * a.dim + d);
+      o[0] = fmaf(v.x, f, o[0]);
+      o[1] = fmaf(v.y, f, o[1]);
+      o[2] = fmaf(v.z, f, o[2]);
+      o[3] = fmaf(v.w, f, o[3]);
+    }
+  }
+  const bool some = l != 0.f;                // a NaN is some, too
+  if (d < a.dim) {
+    const float inv = some ? 1.0f / l : 0.f;
+    *reinterpret_cast<uint2*>(a.out + token * a.out_token + head * a.out_head + d) =
+        make_uint2(bf16_pair(o[0] * inv, o[1] * inv), bf16_pair(o[2] * inv, o[3] * inv));
+  }
+  if (a.lse != nullptr && lane == 0) a.lse[at] = some ? base + logf(l) : -INFINITY;
+}
+
+int device_sms() {
+  static int sms[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (sms[dev] == 0) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    sms[dev] = n;
+  }
+  return sms[dev];
+}
+
+struct Plan {
+  int pack_log2, groups, chunk, chunks_most;
+  int64_t grid;
+};
+
+// How a call is cut up.  Only its sizes are known here, not its offsets.
+Plan plan_of(const AttnParams& a, int sms) {
+  Plan plan = {};
+  const int group = a.heads / a.kv_heads;
+  while (plan.pack_log2 < 7 && group % (2 << plan.pack_log2) == 0) ++plan.pack_log2;
+  plan.groups = a.heads >> plan.pack_log2;
+  const int64_t pair_tokens = 2 * (kTile >> plan.pack_log2);
+  const int64_t pairs = a.tokens_q / pair_tokens + (a.tokens_q < a.sequences ? a.tokens_q : a.sequences);   // at most
+  const int64_t items = pairs * plan.groups;
+  const int64_t tiles = (a.tokens_k + kTile - 1) / kTile;                   // of the longest sequence there can be
+  plan.chunk = (int)(tiles < 1 ? 1 : tiles);
+  plan.chunks_most = 1;
+  if (items < 4 * (int64_t)sms) {
+    // a quarter of a CTA's share each, if the sequences are alike; no fewer than 4 tiles, which a chunk's start would outweigh
+    int64_t chunk = (tiles + a.sequences) * plan.groups * ((pairs + a.sequences - 1) / a.sequences) / (4 * (int64_t)sms);
+    if (chunk < 4) chunk = 4;
+    const int64_t most_bytes = 256ll << 20, row = a.tokens_q * a.heads * (a.dim + 1) * 4;
+    while (chunk < tiles && (tiles + chunk - 1) / chunk * row > most_bytes) chunk *= 2;
+    if (chunk < tiles) {
+      plan.chunk = (int)chunk;
+      plan.chunks_most = (int)((tiles + chunk - 1) / chunk);
+    }
+  }
+  const int64_t most = items * plan.chunks_most;
+  plan.grid = most < sms ? most : sms;
+  return plan;
+}
+
+int64_t part_lse_offset(const AttnParams& a, const Plan& plan) {
+  return ((int64_t)plan.chunks_most * a.tokens_q * a.heads * a.dim * 4 + 255) / 256 * 256;
+}
+
+bool strides_for_tma(int64_t token, int64_t head, int heads, int64_t tokens) {
+  auto fine = [](int64_t s, int64_t n) { return n == 1 || (s > 0 && s % 8 == 0 && s < (1ll << 38)); };
+  return fine(head, heads) && fine(token, tokens);
+}
+
+}  // namespace
+
+bool attention_tmem_supported(const AttnParams& a) {
+  auto al = [](const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
+  return a.dim <= 128 && a.dim % 8 == 0 && a.tokens_k > 0 && al(a.q, 16) && al(a.k, 16) && al(a.v, 16) && al(a.out, 16) &&
+         a.out_token % 8 == 0 && a.out_head % 8 == 0 && strides_for_tma(a.q_token, a.q_head, a.heads, a.tokens_q) &&
+         strides_for_tma(a.k_token, a.k_head, a.kv_heads, a.tokens_k) && strides_for_tma(a.v_token, a.v_head, a.kv_heads, a.tokens_k);
+}
+
+int64_t attention_tmem_workspace(const AttnParams& a) {
+  const Plan plan = plan_of(a, device_sms());
+  return plan.chunks_most == 1 ? 0 : part_lse_offset(a, plan) + (int64_t)plan.chunks_most * a.tokens_q * a.heads * 4;
+}
+
+int attention_tmem_status(int* out) {
+  SACQ_CUDA_TRY(cudaMemcpyFromSymbol(out, g_status, sizeof(int)));
+  return SACQ_OK;
+}
+
+int launch_attention_tmem(const AttnParams& a, void* workspace, int64_t workspace_bytes, cudaStream_t s) {
+  const Plan plan = plan_of(a, device_sms());
+  TmemAttnParams p = {};
+  p.a = a;
+  p.pack_log2 = plan.pack_log2;
+  p.groups = plan.groups;
+  p.chunk = plan.chunk;
+  p.chunks_most = plan.chunks_most;
+  if (plan.chunks_most > 1) {
+    const int64_t need = attention_tmem_workspace(a);
+    if (workspace == nullptr || workspace_bytes < need)
+      return set_error(SACQ_ERR_WORKSPACE, "workspace of %lld bytes, %lld are needed", (long long)(workspace ? workspace_bytes : 0), (long long)need);
+    if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return set_error(SACQ_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
+    p.part_o = static_cast<float*>(workspace);
+    p.part_lse = reinterpret_cast<float*>(static_cast<char*>(workspace) + part_lse_offset(a, plan));
+  }
+  // the stride of a dimension of one element means nothing, but is checked
+  auto stride = [](int64_t s, int64_t n, int64_t other) { return n == 1 ? other : s; };
+  CUtensorMap mq, mk, mv;
+  const int pack = 1 << plan.pack_log2;
+  const int64_t dim8 = a.dim;
+  auto make = [&](CUtensorMap* m, const void* base, int64_t tokens, int heads, int64_t token, int64_t head, int box_heads, int box_tokens) {
+    const int64_t h = stride(head, heads, dim8), t = stride(token, tokens, dim8 * heads);
+    return encode_bf16_3d(m, base, (uint64_t)a.dim, (uint64_t)heads, (uint64_t)tokens, (uint64_t)h, (uint64_t)t, 64u, (uint32_t)box_heads, (uint32_t)box_tokens,
+                          CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  int rc = make(&mq, a.q, a.tokens_q, a.heads, a.q_token, a.q_head, pack, kTile / pack);
+  if (rc == SACQ_OK) rc = make(&mk, a.k, a.tokens_k, a.kv_heads, a.k_token, a.k_head, 1, kTile);
+  if (rc == SACQ_OK) rc = make(&mv, a.v, a.tokens_k, a.kv_heads, a.v_token, a.v_head, 1, kTile);
+  if (rc != SACQ_OK) return rc;
+  const bool wide = a.dim > 64;
+  const void* fn = wide ? (const void*)attention_tmem_kernel<128> : (const void*)attention_tmem_kernel<64>;
+  const size_t smem = (wide ? Shape<128>::kTotal : Shape<64>::kTotal) + 1024;
+  static bool configured[2][64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[wide][dev]) {
+    SACQ_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (dev >= 0 && dev < 64) configured[wide][dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)plan.grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  void* args[] = {&mq, &mk, &mv, &p};
+  SACQ_CUDA_TRY(cudaLaunchKernelExC(&cfg, fn, args));
+  count_launch();
+  if (plan.chunks_most > 1) {
+    const int64_t grid = (a.tokens_q * a.heads + 3) / 4;
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = 0;
+    void* join_args[] = {&p};
+    SACQ_CUDA_TRY(cudaLaunchKernelExC(&cfg, (const void*)attention_join_kernel, join_args));
+    count_launch();
+  }
+  return SACQ_OK;
+}
+
+}  // namespace sacq

@@ -84,25 +84,17 @@ int check_attention(const sacq_attention_desc* d) {
   if (d->heads % d->kv_heads != 0)
     return set_error(SACQ_ERR_INVALID_ARGUMENT, "%d heads are no multiple of %d key-value heads", d->heads, d->kv_heads);
   if (d->head_dim > 256) return set_error(SACQ_ERR_UNSUPPORTED, "head_dim=%d above 256", d->head_dim);
-  if (d->tokens_q > 2147483647LL || d->tokens_k > 2147483647LL || d->heads > 65536)
-    return set_error(SACQ_ERR_UNSUPPORTED, "more than 2^31 - 1 tokens or 65,536 heads");
+  if (d->tokens_q > 2147480000LL || d->tokens_k > 2147480000LL || d->heads > 65536)
+    return set_error(SACQ_ERR_UNSUPPORTED, "more than 2,147,480,000 tokens or 65,536 heads");
   if (!(d->scale > 0.f) || isinf(d->scale)) return set_error(SACQ_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
   return SACQ_OK;
 }
 
 }  // namespace
 
-SACQ_API int64_t sacq_attention_workspace_bytes(const sacq_attention_desc* d) {
-  if (check_attention(d) != SACQ_OK) return -1;
-  return 0;
-}
+namespace {
 
-SACQ_API int sacq_attention_packed(const sacq_attention_desc* d, void* stream) {
-  if (int rc = check_attention(d)) return rc;
-  if (d->tokens_q == 0 || d->sequences == 0) return SACQ_OK;
-  if (d->q == nullptr || d->out == nullptr || d->cu_q == nullptr || d->cu_k == nullptr ||
-      (d->tokens_k > 0 && (d->k == nullptr || d->v == nullptr)))
-    return set_error(SACQ_ERR_INVALID_ARGUMENT, "null argument");
+AttnParams attention_params(const sacq_attention_desc* d) {
   AttnParams p = {};
   p.q = static_cast<const uint16_t*>(d->q);
   p.k = static_cast<const uint16_t*>(d->k);
@@ -118,5 +110,30 @@ SACQ_API int sacq_attention_packed(const sacq_attention_desc* d, void* stream) {
   p.sequences = d->sequences; p.heads = d->heads; p.kv_heads = d->kv_heads; p.dim = d->head_dim;
   p.causal = d->causal != 0;
   p.scale = d->scale;
+  return p;
+}
+
+}  // namespace
+
+SACQ_API int64_t sacq_attention_workspace_bytes(const sacq_attention_desc* d) {
+  if (int rc = check_attention(d)) return rc;
+  if (d->tokens_q == 0 || d->sequences == 0) return 0;
+  const AttnParams p = attention_params(d);
+  return attention_tmem_supported(p) ? attention_tmem_workspace(p) : 0;
+}
+
+SACQ_API int sacq_attention_packed(const sacq_attention_desc* d, void* stream) {
+  if (int rc = check_attention(d)) return rc;
+  if (d->tokens_q == 0 || d->sequences == 0) return SACQ_OK;
+  if (d->q == nullptr || d->out == nullptr || d->cu_q == nullptr || d->cu_k == nullptr ||
+      (d->tokens_k > 0 && (d->k == nullptr || d->v == nullptr)))
+    return set_error(SACQ_ERR_INVALID_ARGUMENT, "null argument");
+  const AttnParams p = attention_params(d);
+  if (attention_tmem_supported(p)) return launch_attention_tmem(p, d->workspace, d->workspace_bytes, static_cast<cudaStream_t>(stream));
   return launch_attention_rows(p, static_cast<cudaStream_t>(stream));
+}
+
+SACQ_API int sacq_attention_status(int* status_out) {
+  if (status_out == nullptr) return set_error(SACQ_ERR_INVALID_ARGUMENT, "null argument");
+  return attention_tmem_status(status_out);
 }

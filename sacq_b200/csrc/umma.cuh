@@ -160,6 +160,9 @@ __host__ __device__ constexpr uint32_t make_idesc_i8(int bn) {
 // 2-D byte tensor [rows][row_bytes] with a [box_rows][box_bytes] box (linear_large_m.cu).
 int encode_bytes_2d(CUtensorMap* map, const void* base, uint64_t row_bytes, uint64_t rows, uint64_t pitch_bytes,
                     uint32_t box_bytes, uint32_t box_rows, CUtensorMapSwizzle swizzle);
+// 3-D bf16 tensor [n2][n1][n0] with strides in elements and a [box2][box1][box0] box (linear_large_m.cu).
+int encode_bf16_3d(CUtensorMap* map, const void* base, uint64_t n0, uint64_t n1, uint64_t n2, uint64_t stride1, uint64_t stride2, uint32_t box0,
+                   uint32_t box1, uint32_t box2, CUtensorMapSwizzle swizzle);
 
 // Tile map over a layer's packed index rows: box = one index super-block (two 128-k blocks) x
 // 128 weight rows.  Built on first use and kept by the layer.
