@@ -393,7 +393,7 @@ SACQ_API int sacq_attention_packed(const sacq_attention_desc* desc, void* stream
 SACQ_API int64_t sacq_attention_workspace_bytes(const sacq_attention_desc* desc);
 /* Reads the current device's status word of these kernels (synchronises the device): 0, or a nonzero code written by one
  * whose bounded wait gave up. */
-SACQ_API int sacq_attention_status(int* status_out);
+SACQ_API int sacq_block_steps_status(int* status_out);
 
 /* Forces a GEMM kernel (for tests and benchmarks): 0 = automatic, 1 = small-M kernel
  * (its own choice of variant), 2 = tensor-core kernel that splits K over clusters, 3 = small-M

@@ -128,7 +128,7 @@ SIGNATURES = {
     "sacq_residual_norm": (_int, [ctypes.POINTER(ResidualNormDesc), _vp]),
     "sacq_attention_packed": (_int, [ctypes.POINTER(AttentionDesc), _vp]),
     "sacq_attention_workspace_bytes": (_i64, [ctypes.POINTER(AttentionDesc)]),
-    "sacq_attention_status": (_int, [ctypes.POINTER(_int)]),
+    "sacq_block_steps_status": (_int, [ctypes.POINTER(_int)]),
     "sacq_layer_set_kernel": (_int, [_vp, _int]),
     "sacq_layer_set_shard_of": (_int, [_vp, _i64]),
     "sacq_layer_kernel_for": (_int, [_vp, _i64]),

@@ -9,6 +9,7 @@ namespace sacq {
 
 int launch_rotate_heads(const sacq_rotary_desc& d, cudaStream_t s);
 int launch_residual_norm(const sacq_residual_norm_desc& d, cudaStream_t s);
+int residual_norm_status(int* out);
 
 namespace {
 
@@ -133,7 +134,11 @@ SACQ_API int sacq_attention_packed(const sacq_attention_desc* d, void* stream) {
   return launch_attention_rows(p, static_cast<cudaStream_t>(stream));
 }
 
-SACQ_API int sacq_attention_status(int* status_out) {
+SACQ_API int sacq_block_steps_status(int* status_out) {
   if (status_out == nullptr) return set_error(SACQ_ERR_INVALID_ARGUMENT, "null argument");
-  return attention_tmem_status(status_out);
+  int norm = 0;
+  if (int rc = attention_tmem_status(status_out)) return rc;
+  if (int rc = residual_norm_status(&norm)) return rc;
+  *status_out |= norm;
+  return SACQ_OK;
 }
