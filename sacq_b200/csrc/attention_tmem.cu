@@ -20,6 +20,7 @@
 #include <cuda.h>
 
 #include "attention.cuh"
+#include "encode.cuh"
 #include "umma.cuh"
 
 namespace sacq {
@@ -75,8 +76,8 @@ struct Shape {
   static constexpr int kS = 0, kO = 256;
 };
 // mbarriers
-constexpr int Q_FULL = 0, Q_EMPTY = 1, S_FULL = 2, P_FULL = 4, O_FULL = 6, ITEM_FULL = 8, ITEM_EMPTY = 10, DRAIN = 12,
-              KV_FULL = 16, KV_EMPTY = 32, JOIN_FULL = 48, JOIN_EMPTY = 52;
+constexpr int Q_FULL = 0, Q_EMPTY = 1, S_FULL = 2, P_FULL = 4, O_FULL = 6, ITEM_FULL = 10, ITEM_EMPTY = 12,
+              DRAIN = 14, KV_FULL = 16, KV_EMPTY = 32, JOIN_FULL = 48, JOIN_EMPTY = 52;
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -141,15 +142,77 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {      // without waiting
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :: "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// The largest of three, NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x of two values: on the special-function unit, or by a polynomial.  The unit takes 8 cycles for a warp, which would
+// bound the kernel; of every 8 pairs kPolynomials go by x = n + f, f in [-1/2, 1/2], and a polynomial of degree 5 for 2^f (least
+// largest relative error, 7.5e-8, fitted by iterated reweighted least squares), n added to its exponent.  Below 2^-126 the
+// result is that power: such weights count for nothing beside the row's largest.
+constexpr int kPolynomials = 2;
+__device__ __forceinline__ uint64_t exp2_unit(uint64_t v) {
+  float x, y;
+  halves_of(v, x, y);
+  return f32x2(exp2_fast(x), exp2_fast(y));
+}
+__device__ __forceinline__ uint64_t exp2_polynomial(uint64_t v) {
+  float x, y;
+  halves_of(v, x, y);
+  v = f32x2(fmaxf(x, -126.f), fmaxf(y, -126.f));
+  const uint64_t magic = f32x2(12582912.0f, 12582912.0f);            // 1.5 * 2^23: the sum holds the nearest integer in its low bits
+  const uint64_t t = add2(v, magic);
+  const uint64_t f = fma2(add2(t, f32x2(-12582912.0f, -12582912.0f)), f32x2(-1.f, -1.f), v);
+  uint64_t r = fma2(f32x2(0.0013276472454890609f, 0.0013276472454890609f), f, f32x2(0.009675541892647743f, 0.009675541892647743f));
+  r = fma2(r, f, f32x2(0.05550713092088699f, 0.05550713092088699f));
+  r = fma2(r, f, f32x2(0.24022120237350464f, 0.24022120237350464f));
+  r = fma2(r, f, f32x2(0.6931469440460205f, 0.6931469440460205f));
+  r = fma2(r, f, f32x2(1.0000001192092896f, 1.0000001192092896f));
+  float a, b, ta, tb;
+  halves_of(r, a, b);
+  halves_of(t, ta, tb);
+  return f32x2(__uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23)), __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23)));
+}
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+// An item's fields, the same in all lanes and known to be: what is computed from them may stay in uniform registers.
+__device__ __forceinline__ Item uniform_item(const Item* at) {
+  Item it;
+#define SACQ_SAME(field) it.field = (int)warp_uniform((uint32_t)at->field)
+  SACQ_SAME(last); SACQ_SAME(q_row); SACQ_SAME(q_left); SACQ_SAME(head); SACQ_SAME(kv_head); SACQ_SAME(k_row); SACQ_SAME(keys);
+  SACQ_SAME(base); SACQ_SAME(n); SACQ_SAME(n0); SACQ_SAME(dual); SACQ_SAME(part);
+#undef SACQ_SAME
+  return it;
 }
 // Keys that token t of an item sees.
 __device__ __forceinline__ int seen(const Item& it, bool causal, int t) { return causal ? max(0, min(it.keys, it.base + t + 1)) : it.keys; }
@@ -188,7 +251,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   Item* const items = reinterpret_cast<Item*>(sp + Sh::kItems);       // two of 64 bytes
   auto item_at = [&](uint32_t i) { return reinterpret_cast<Item*>(reinterpret_cast<uint8_t*>(items) + (i & 1) * 64); };
   auto bar = [&](int i) { return sm + Sh::kBars + 8u * i; };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = (int)warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const AttnParams& a = p.a;
   const int tokens_log2 = 7 - p.pack_log2;                              // tokens of a tile
   const int tile_tokens = 1 << tokens_log2;
@@ -228,7 +291,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = warp_uniform(*tmem_slot);
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   if (warp == kLoadWarp) {
@@ -313,11 +376,10 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       }
       ok = mbar_wait_warp(bar(ITEM_EMPTY + (made & 1)), ((made >> 1) & 1) ^ 1, abort_flag, &g_status);
       if (!ok) break;
-      if (lane == 0) {
-        *item_at(made) = it;
-        mbar_arrive(bar(ITEM_FULL + (made & 1)));
-      }
+      if (lane == 0) *item_at(made) = it;
       __syncwarp();
+      it = uniform_item(item_at(made));
+      if (lane == 0) mbar_arrive(bar(ITEM_FULL + (made & 1)));
       ++made;
       if (it.last) break;
       if (it.n == 0) continue;
@@ -344,16 +406,15 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         for (int t = 0; t < 100000 && !mbar_try_wait(bar(KV_FULL + i % Sh::kStages), (i / Sh::kStages) & 1); ++t) {}
   } else if (warp == kMmaWarp) {
     // ---- MMA issuer
-    uint32_t c = 0, nq = 0, np[2] = {0, 0};
+    uint32_t c = 0, nq = 0, np0 = 0, np1 = 0;           // ring tiles, items with keys, products of each warpgroup
     const int k_steps = (a.dim + 15) / 16;
-    const uint32_t pv_n = (uint32_t)k_steps * 16;
-    const uint32_t idesc_pv = idesc_bf16((int)pv_n, true);
+    const uint32_t idesc_pv = idesc_bf16(k_steps * 16, true);
     bool ok = true;
     auto next = [&]() -> uint32_t {          // the next tile of the ring
       const uint32_t s = c % Sh::kStages;
       ok = ok && mbar_wait_warp(bar(KV_FULL + s), (c / Sh::kStages) & 1, abort_flag, &g_status);
       ++c;
-      return s;
+      return warp_uniform(s);
     };
     auto commit = [&](int b) {
       if (elect_one()) umma_commit(bar(b));
@@ -362,29 +423,29 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     auto qk = [&](int w, int tile, uint32_t s, int n) {       // S of warpgroup w from Q tile `tile`
       if (!ok) return;
       const uint32_t idesc = warp_uniform(idesc_bf16(n, false));
-      const uint32_t q0 = sm + Sh::kQ + tile * Sh::kTileBytes, k0 = sm + Sh::kRing + s * Sh::kTileBytes;
-      if (elect_one()) {
+      const uint64_t qd = make_smem_desc(sm + Sh::kQ + tile * Sh::kTileBytes), kd = make_smem_desc(sm + Sh::kRing + s * Sh::kTileBytes);
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-          const uint32_t off = (i >> 2) * Sh::kHalfBytes + (i & 3) * 32;
-          if (i < k_steps) umma_bf16_ss(tmem + Sh::kS + w * kTile, make_smem_desc(q0 + off), make_smem_desc(k0 + off), idesc, i > 0);
-        }
+      for (int i = 0; i < DP / 16; ++i) {
+        const uint64_t adv = (uint64_t)(((i >> 2) * Sh::kHalfBytes + (i & 3) * 32) >> 4);
+        if (i < k_steps && elect_one()) umma_bf16_ss(tmem + Sh::kS + w * kTile, qd + adv, kd + adv, idesc, i > 0);
       }
       __syncwarp();
     };
-    auto pv = [&](int w, uint32_t s, int n, bool first) {     // O of warpgroup w += P V over the tile's first n keys
-      ok = ok && mbar_wait_warp(bar(P_FULL + w), np[w] & 1, abort_flag, &g_status);
-      ++np[w];
+    // O of warpgroup w += P V over the tile's first n keys.  (What the instructions are issued with has to be in uniform
+    // registers, and the warp converged in front of and behind each group: 120 clocks each otherwise, 64 so.)
+    auto pv = [&](int w, uint32_t s, int n, bool first) {
+      n = (int)warp_uniform(n); w = (int)warp_uniform(w); s = warp_uniform(s);
+      const uint64_t vd = make_mn_desc(sm + Sh::kRing + s * Sh::kTileBytes, Sh::kHalfBytes);
+      const uint32_t more = warp_uniform(first ? 0u : 1u);
+      ok = ok && mbar_wait_warp(bar(P_FULL + w), (w == 0 ? np0 : np1) & 1, abort_flag, &g_status);
       if (!ok) return;
       tc_fence_after();
-      const uint32_t v0 = sm + Sh::kRing + s * Sh::kTileBytes;
-      if (elect_one()) {
 #pragma unroll
-        for (int i = 0; i < kTile / 16; ++i)
-          if (i * 16 < n)
-            umma_bf16_ts(tmem + Sh::kO + w * DP, tmem + Sh::kS + w * kTile + i * 8, make_mn_desc(v0 + i * 2048, Sh::kHalfBytes), idesc_pv, !first || i > 0);
-      }
+      for (int i = 0; i < kTile / 16; ++i)
+        if (i * 16 < n && elect_one())
+          umma_bf16_ts(tmem + Sh::kO + w * DP, tmem + Sh::kS + w * kTile + i * 8, vd + (uint64_t)(i * 2048 >> 4), idesc_pv, i > 0 ? 1u : more);
       __syncwarp();
+      if (w == 0) ++np0; else ++np1;
     };
     // rows of a V tile behind the last key, up to a whole instruction: zeros, whatever lies there in memory
     auto clear_tail = [&](uint32_t s, int keys) {
@@ -399,8 +460,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     };
     for (uint32_t i = 0; ok; ++i) {
       if (!mbar_wait_warp(bar(ITEM_FULL + (i & 1)), (i >> 1) & 1, abort_flag, &g_status)) break;
-      const Item it = *item_at(i);
-      __syncwarp();
+      const Item it = uniform_item(item_at(i));
       if (lane == 0) mbar_arrive(bar(ITEM_EMPTY + (i & 1)));
       if (it.last) break;
       if (it.n == 0) continue;
@@ -481,8 +541,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     bool ok = true;
     for (uint32_t i = 0; ok; ++i) {
       if (!mbar_wait_warp(bar(ITEM_FULL + (i & 1)), (i >> 1) & 1, abort_flag, &g_status)) break;
-      const Item it = *item_at(i);
-      __syncwarp();
+      const Item it = uniform_item(item_at(i));
       if (lane == 0) mbar_arrive(bar(ITEM_EMPTY + (i & 1)));
       if (it.last) break;
       const int t = (row >> p.pack_log2) + (it.dual ? w * tile_tokens : 0);      // token of the item
@@ -499,57 +558,74 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         if (live) {
           tc_fence_after();
           uint32_t s[4][32];
+          const int end = mine - j * kTile;
+          const bool masked = (j + 1) * kTile > least;
+          float top[2] = {m, m};
 #pragma unroll
-          for (int b = 0; b < 4; ++b) tmem_ld32(s_at + b * 32, s[b]);
+          for (int h = 0; h < 2; ++h) {      // the second half is fetched while the first one's maximum is taken
+            if (h == 0) {
+              tmem_ld32(s_at, s[0]);
+              tmem_ld32(s_at + 32, s[1]);
+              tmem_wait_ld(s[0]);
+              tmem_wait_ld(s[1]);
+              tmem_ld32(s_at + 64, s[2]);
+              tmem_ld32(s_at + 96, s[3]);
+            } else {
+              tmem_wait_ld(s[2]);
+              tmem_wait_ld(s[3]);
+            }
+            if (masked) {                    // columns that this row does not see
 #pragma unroll
-          for (int b = 0; b < 4; ++b) tmem_wait_ld(s[b]);
-          if ((j + 1) * kTile > least) {     // columns that this row does not see
-            const int end = mine - j * kTile;
+              for (int b = 2 * h; b < 2 * h + 2; ++b)
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
+                for (int e = 0; e < 32; ++e)
+                  if (b * 32 + e >= end) s[b][e] = 0xff800000u;
+            }
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (b * 32 + e >= end) s[b][e] = 0xff800000u;
+            for (int b = 2 * h; b < 2 * h + 2; ++b)
+#pragma unroll
+              for (int e = 0; e < 32; e += 2)
+                top[b & 1] = max_nan(top[b & 1], __uint_as_float(s[b][e]), __uint_as_float(s[b][e + 1]));
           }
-          float top[4];
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            top[b] = __uint_as_float(s[b][0]);
-#pragma unroll
-            for (int e = 1; e < 32; ++e) top[b] = fmaxf(top[b], __uint_as_float(s[b][e]));
-          }
-          const float high = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
-          if (__any_sync(0xffffffffu, (high - m) * c2 > kRescale)) {
+          const float high = max_nan(top[0], top[1], top[1]);
+          if (__any_sync(0xffffffffu, !((high - m) * c2 <= kRescale))) {      // NaN: yes
             const float keep = m == -INFINITY ? 0.f : exp2_fast((m - high) * c2);
             m = high;
             l *= keep;
             if (!first) {
 #pragma unroll 1
-              for (int b = 0; b < DP / 32; ++b) {
-                uint32_t o[32];
-                tmem_ld32(o_at + b * 32, o);
-                tmem_wait_ld(o);
+              for (int b = 0; b < DP / 16; ++b) {
+                uint32_t o[16];
+                tmem_ld16(o_at + b * 16, o);
+                tmem_wait_ld16(o);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                tmem_st32(o_at + b * 32, o);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                tmem_st16(o_at + b * 16, o);
               }
             }
           }
-          const float base = m == -INFINITY ? 0.f : m * c2;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          // a row whose maximum is infinite or NaN is NaN: the weights of the special-function unit are
+          const float base = m == -INFINITY ? 0.f : fabsf(m) < INFINITY ? -m * c2 : __uint_as_float(0x7fc00000u);
+          const uint64_t scale2 = f32x2(c2, c2), base2 = f32x2(base, base);
+          uint64_t sum[2] = {f32x2(0.f, 0.f), f32x2(0.f, 0.f)};
 #pragma unroll
-          for (int b = 0; b < 4; b += 2) {
-            uint32_t w2[32];
+          for (int h = 0; h < 2; ++h) {
+            uint32_t weights[32];
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
-              const float x = exp2_fast(fmaf(__uint_as_float(s[b + (e >> 4)][2 * (e & 15)]), c2, -base));
-              const float y = exp2_fast(fmaf(__uint_as_float(s[b + (e >> 4)][2 * (e & 15) + 1]), c2, -base));
-              sum[e & 3] += x + y;
-              w2[e] = bf16_pair(x, y);
+              const uint32_t* const pair = &s[2 * h + (e >> 4)][2 * (e & 15)];
+              const uint64_t t = fma2(f32x2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), scale2, base2);
+              const uint64_t w2 = e % 8 < kPolynomials ? exp2_polynomial(t) : exp2_unit(t);
+              float x, y;
+              halves_of(w2, x, y);
+              sum[e & 1] = add2(sum[e & 1], w2);
+              weights[e] = bf16_pair(x, y);
             }
-            tmem_st32(s_at + b * 16, w2);
+            tmem_st32(s_at + h * 32, weights);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          float x, y;
+          halves_of(add2(sum[0], sum[1]), x, y);
+          l += x + y;
           tmem_wait_st();
           first = false;
         }
