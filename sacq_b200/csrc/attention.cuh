@@ -4,6 +4,8 @@
 // aligned (j <= i + keys - queries).  A query that sees none has out = 0 and lse = -inf.
 #pragma once
 
+#include <cuda.h>
+
 #include "common.cuh"
 
 namespace sacq {
@@ -63,12 +65,127 @@ __device__ void attend_row(const AttnParams& p, const uint16_t* q, const uint16_
   }
 }
 
-int launch_attention_rows(const AttnParams& p, cudaStream_t s);          // any head dim up to 256, any alignment
+// A call that is cut up: chunks of `chunk` key tiles whose results, with their own lse, a second kernel joins.
+constexpr int kKeyTile = 128;
+struct AttnSplit {
+  int chunk, chunks_most;          // chunks of the longest sequence possible; 1: results go straight to out
+  float* part_o;                   // [chunks_most][tokens_q][heads][dim]
+  float* part_lse;                 // [chunks_most][tokens_q][heads]
+};
+__host__ __device__ __forceinline__ int key_tiles(int keys) { return (keys + kKeyTile - 1) / kKeyTile; }
+__device__ __forceinline__ int chunks_of(const AttnSplit& s, int keys) {
+  const int n = (key_tiles(keys) + s.chunk - 1) / s.chunk;
+  return s.chunks_most > 1 && n > 1 ? n : 1;
+}
 
-// Tensor cores: head dims that are multiples of 8 up to 128, rows that TMA can read.
-bool attention_tmem_supported(const AttnParams& p);
-int64_t attention_tmem_workspace(const AttnParams& p);
-int attention_tmem_status(int* out);
-int launch_attention_tmem(const AttnParams& p, void* workspace, int64_t workspace_bytes, cudaStream_t s);
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+               : "memory");
+}
+
+// One output row by a warp, for rows that a non-finite value of a key they do not see got into (0 x inf): the keys that they
+// see, one after another.  part: the chunk, or -1; elements [from, to) are written.
+__device__ __noinline__ inline void redo_row(const AttnParams& a, const AttnSplit& split, int k_row, int kv_head, int part, int64_t token, int head,
+                                             int keys, int from, int to) {
+  const int lane = threadIdx.x & 31;
+  RowState<4> st;
+  attend_row<4>(a, a.q + token * a.q_token + head * a.q_head, a.k + k_row * a.k_token + kv_head * a.k_head,
+                a.v + k_row * a.v_token + kv_head * a.v_head, keys, st);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int d = lane + 32 * e;
+    if (d >= a.dim || d < from || d >= to) continue;
+    const float o = st.acc[e] / st.l;
+    if (part < 0) a.out[token * a.out_token + head * a.out_head + d] = float_to_bf16_bits(o);
+    else split.part_o[(((int64_t)part * a.tokens_q + token) * a.heads + head) * a.dim + d] = o;
+  }
+}
+
+// Items of work, sequence after sequence, listed by one warp: 32 sequences are looked at at a time.  count(queries, keys) is how
+// many items a sequence has.
+template <typename Count>
+struct ItemList {
+  const AttnParams& a;
+  Count count;
+  int window = 0;
+  int64_t before = 0, mine = 0, upto = 0;      // items in front of the window; this lane's sequence's, and up to it
+  Span sq = {0, 0}, sk = {0, 0};
+  __device__ __forceinline__ void look() {
+    const int lane = threadIdx.x & 31, s = window + lane;
+    mine = 0;
+    sq = sk = {0, 0};
+    if (s < a.sequences) {
+      sq = span_of(a.cu_q, s, a.tokens_q);
+      sk = span_of(a.cu_k, s, a.tokens_k);
+      mine = count((int)sq.length, (int)sk.length);
+    }
+    upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+  }
+  // The sequence of item `index` (not smaller than the last one asked for), and which of its items that is; false: there is none.
+  __device__ __forceinline__ bool find(int64_t index, Span& q, Span& k, int64_t& which) {
+    int64_t all = __shfl_sync(0xffffffffu, upto, 31);
+    while (window < a.sequences && index >= before + all) {
+      before += all;
+      window += 32;
+      look();
+      all = __shfl_sync(0xffffffffu, upto, 31);
+    }
+    const uint32_t found = __ballot_sync(0xffffffffu, index < before + upto);
+    if (window >= a.sequences || found == 0) return false;
+    const int src = __ffs(found) - 1;
+    q = {__shfl_sync(0xffffffffu, sq.begin, src), __shfl_sync(0xffffffffu, sq.length, src)};
+    k = {__shfl_sync(0xffffffffu, sk.begin, src), __shfl_sync(0xffffffffu, sk.length, src)};
+    which = index - (before + __shfl_sync(0xffffffffu, upto, src) - __shfl_sync(0xffffffffu, mine, src));
+    return true;
+  }
+};
+
+// The next digit of `r` in base `n`; r is left with the rest.  (A 64-bit division takes about 100 instructions.)
+__device__ __forceinline__ int digit_of(int64_t& r, int n) {
+  if (r >> 32 == 0) {
+    const uint32_t x = (uint32_t)r, y = x / (uint32_t)n;
+    r = y;
+    return (int)(x - y * (uint32_t)n);
+  }
+  const int d = (int)(r % n);
+  r /= n;
+  return d;
+}
+
+int launch_attention_rows(const AttnParams& p, cudaStream_t s);          // any head dim up to 256, any alignment
+int launch_attention_join(const AttnParams& a, const AttnSplit& split, cudaStream_t s);
+
+// Head dims that are multiples of 8 up to 128, rows that TMA can read.
+bool attention_tma_supported(const AttnParams& p);
+// How a call is cut up for a kernel with `slots` CTAs at once: `items` pieces of work without a cut.
+AttnSplit attention_split(const AttnParams& a, int64_t items, int64_t items_per_sequence, int64_t slots, int min_chunk, void* workspace);
+int64_t attention_split_bytes(const AttnParams& a, const AttnSplit& split);
+int attention_tensor_maps(const AttnParams& a, int q_box_heads, int q_box_tokens, int k_box_tokens, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v);
+int device_sms();
+
+// Tensor cores by tcgen05: tiles of 128 query rows.
+AttnSplit attention_tmem_split(const AttnParams& p, void* workspace);
+int launch_attention_tmem(const AttnParams& p, const AttnSplit& split, cudaStream_t s);
+// Tensor cores by mma.sync: tiles of 16 query rows.
+AttnSplit attention_short_split(const AttnParams& p, void* workspace);
+int launch_attention_short(const AttnParams& p, const AttnSplit& split, cudaStream_t s);
+int attention_status(int* out);
+int* attention_status_word();
 
 }  // namespace sacq

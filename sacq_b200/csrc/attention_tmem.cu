@@ -29,22 +29,17 @@ namespace {
 
 using namespace umma;
 
-constexpr int kTile = 128;
+constexpr int kTile = kKeyTile;
 constexpr int kThreads = 320;
 constexpr int kMmaWarp = 8, kLoadWarp = 9;
 constexpr float kRescale = 8.0f;            // log2
-constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ int g_status;                    // nonzero: a wait ran out
 
 struct TmemAttnParams {
   AttnParams a;
   int pack_log2;                            // heads of a tile
   int groups;                               // heads / pack
-  int chunk;                                // key tiles of a chunk
-  int chunks_most;                          // chunks of the longest sequence possible; 1: results go straight to out
-  float* part_o;                            // [chunks_most][tokens_q][heads][dim]
-  float* part_lse;                          // [chunks_most][tokens_q][heads]
+  AttnSplit split;
+  int* status;
 };
 
 struct Item {
@@ -79,11 +74,6 @@ struct Shape {
 constexpr int Q_FULL = 0, Q_EMPTY = 1, S_FULL = 2, P_FULL = 4, O_FULL = 6, ITEM_FULL = 10, ITEM_EMPTY = 12,
               DRAIN = 14, KV_FULL = 16, KV_EMPTY = 32, JOIN_FULL = 48, JOIN_EMPTY = 52;
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
-               : "memory");
-}
 __device__ __forceinline__ void umma_bf16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -163,11 +153,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // The largest of three, NaN if one is.
 __device__ __forceinline__ float max_nan(float a, float b, float c) {
   float r;
@@ -201,10 +186,6 @@ __device__ __forceinline__ uint64_t exp2_polynomial(uint64_t v) {
   halves_of(t, ta, tb);
   return f32x2(__uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23)), __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23)));
 }
-__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
 // An item's fields, the same in all lanes and known to be: what is computed from them may stay in uniform registers.
 __device__ __forceinline__ Item uniform_item(const Item* at) {
   Item it;
@@ -216,27 +197,8 @@ __device__ __forceinline__ Item uniform_item(const Item* at) {
 }
 // Keys that token t of an item sees.
 __device__ __forceinline__ int seen(const Item& it, bool causal, int t) { return causal ? max(0, min(it.keys, it.base + t + 1)) : it.keys; }
-__device__ __forceinline__ int key_tiles(int keys) { return (keys + kTile - 1) / kTile; }
 // Columns of key tile j that the tile's last token sees, in whole instructions of 16.
 __device__ __forceinline__ int columns(int most, int j) { return (min(kTile, most - j * kTile) + 15) & ~15; }
-
-// One output row by a warp, for rows that a non-finite value of a key they do not see got into (0 x inf): the keys that they
-// see, one after another.
-__device__ __noinline__ void redo_row(const TmemAttnParams& p, const Item& it, int64_t token, int head, int keys) {
-  const AttnParams& a = p.a;
-  const int lane = threadIdx.x & 31;
-  RowState<4> st;
-  attend_row<4>(a, a.q + token * a.q_token + head * a.q_head, a.k + it.k_row * a.k_token + it.kv_head * a.k_head,
-                a.v + it.k_row * a.v_token + it.kv_head * a.v_head, keys, st);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int d = lane + 32 * e;
-    if (d >= a.dim) continue;
-    const float o = st.acc[e] / st.l;
-    if (it.part < 0) a.out[token * a.out_token + head * a.out_head + d] = float_to_bf16_bits(o);
-    else p.part_o[(((int64_t)it.part * a.tokens_q + token) * a.heads + head) * a.dim + d] = o;
-  }
-}
 
 template <int DP>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -300,7 +262,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     bool ok = true;
     auto take = [&](const CUtensorMap* map, const Item& it, int j) {
       const uint32_t s = c % Sh::kStages;
-      ok = ok && mbar_wait_warp(bar(KV_EMPTY + s), ((c / Sh::kStages) & 1) ^ 1, abort_flag, &g_status);
+      ok = ok && mbar_wait_warp(bar(KV_EMPTY + s), ((c / Sh::kStages) & 1) ^ 1, abort_flag, p.status);
       if (!ok) return;
       if (elect_one()) {
         mbar_arrive_expect_tx(bar(KV_FULL + s), Sh::kTileBytes);
@@ -310,71 +272,39 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       __syncwarp();
       ++c;
     };
-    // sequences are looked at 32 at a time: this lane's number of items and the items in front of it
-    int window = 0;
-    int64_t before = 0;                      // items of the sequences in front of the window
-    int64_t mine = 0, upto = 0;
-    Span sq = {0, 0}, sk = {0, 0};
-    int chunks = 1;
-    auto look = [&] {
-      const int s = window + lane;
-      mine = 0;
-      sq = sk = {0, 0};
-      chunks = 1;
-      if (s < a.sequences) {
-        sq = span_of(a.cu_q, s, a.tokens_q);
-        sk = span_of(a.cu_k, s, a.tokens_k);
-        const int64_t pairs = (sq.length + 2 * tile_tokens - 1) >> (tokens_log2 + 1);
-        if (p.chunks_most > 1) chunks = max(1, (int)((key_tiles((int)sk.length) + p.chunk - 1) / p.chunk));
-        mine = pairs * chunks * p.groups;
-      }
-      upto = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
-      }
+    const auto count = [&](int queries, int keys) -> int64_t {
+      return (int64_t)((queries + 2 * tile_tokens - 1) >> (tokens_log2 + 1)) * chunks_of(p.split, keys) * p.groups;
     };
-    look();
+    ItemList<decltype(count)> list{a, count};
+    list.look();
     for (int64_t index = blockIdx.x; ok; index += gridDim.x) {
-      while (window < a.sequences && index >= before + __shfl_sync(0xffffffffu, upto, 31)) {
-        before += __shfl_sync(0xffffffffu, upto, 31);
-        window += 32;
-        look();
-      }
-      const uint32_t found = __ballot_sync(0xffffffffu, index < before + upto);
       Item it = {};
-      it.last = window >= a.sequences || found == 0;
+      Span sq, sk;
+      int64_t r;
+      it.last = !list.find(index, sq, sk, r);
       if (!it.last) {
-        const int src = __ffs(found) - 1;
-        const int64_t sq_begin = __shfl_sync(0xffffffffu, sq.begin, src), lq = __shfl_sync(0xffffffffu, sq.length, src);
-        const int64_t sk_begin = __shfl_sync(0xffffffffu, sk.begin, src), lk = __shfl_sync(0xffffffffu, sk.length, src);
-        const int nchunks = __shfl_sync(0xffffffffu, chunks, src);
-        const int64_t start = before + __shfl_sync(0xffffffffu, upto, src) - __shfl_sync(0xffffffffu, mine, src);
         // heads first, then chunks; the pairs of tiles from the last, longest one to the first
-        int64_t r = index - start;
-        const int pairs = (int)((lq + 2 * tile_tokens - 1) >> (tokens_log2 + 1));
-        const int group = (int)(r % p.groups);
-        r /= p.groups;
-        const int part = (int)(r % nchunks);
-        const int pair = pairs - 1 - (int)(r / nchunks);
+        const int lq = (int)sq.length, lk = (int)sk.length, chunks = chunks_of(p.split, lk);
+        const int pairs = (lq + 2 * tile_tokens - 1) >> (tokens_log2 + 1);
+        const int group = digit_of(r, p.groups), part = digit_of(r, chunks);
+        const int pair = pairs - 1 - (int)r;
         const int t0 = pair * 2 * tile_tokens;
-        const int tiles = key_tiles((int)lk);
-        const int first = part * p.chunk, n = nchunks > 1 ? min(p.chunk, tiles - first) : tiles;
-        it.q_row = (int)(sq_begin + t0);
-        it.q_left = (int)lq - t0;
+        const int tiles = key_tiles(lk);
+        const int first = chunks > 1 ? part * p.split.chunk : 0, n = chunks > 1 ? min(p.split.chunk, tiles - first) : tiles;
+        it.q_row = (int)sq.begin + t0;
+        it.q_left = lq - t0;
         it.head = group << p.pack_log2;
         it.kv_head = it.head / (a.heads / a.kv_heads);
-        it.k_row = (int)sk_begin + (nchunks > 1 ? first * kTile : 0);
-        it.keys = nchunks > 1 ? min((int)lk - first * kTile, n * kTile) : (int)lk;
-        it.base = (int)(lk - lq) + t0 - (nchunks > 1 ? first * kTile : 0);
+        it.k_row = (int)sk.begin + first * kTile;
+        it.keys = min(lk - first * kTile, n * kTile);
+        it.base = lk - lq + t0 - first * kTile;
         it.dual = it.q_left > tile_tokens;
         const int most = seen(it, causal, min(it.q_left, it.dual ? 2 * tile_tokens : tile_tokens) - 1);
         it.n = key_tiles(most);
         it.n0 = it.dual ? key_tiles(seen(it, causal, tile_tokens - 1)) : 0;
-        it.part = nchunks > 1 ? part : -1;
+        it.part = chunks > 1 ? part : -1;
       }
-      ok = mbar_wait_warp(bar(ITEM_EMPTY + (made & 1)), ((made >> 1) & 1) ^ 1, abort_flag, &g_status);
+      ok = mbar_wait_warp(bar(ITEM_EMPTY + (made & 1)), ((made >> 1) & 1) ^ 1, abort_flag, p.status);
       if (!ok) break;
       if (lane == 0) *item_at(made) = it;
       __syncwarp();
@@ -383,7 +313,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       ++made;
       if (it.last) break;
       if (it.n == 0) continue;
-      ok = mbar_wait_warp(bar(Q_EMPTY), (nq & 1) ^ 1, abort_flag, &g_status);
+      ok = mbar_wait_warp(bar(Q_EMPTY), (nq & 1) ^ 1, abort_flag, p.status);
       if (!ok) break;
       ++nq;
       if (elect_one()) {
@@ -412,7 +342,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     bool ok = true;
     auto next = [&]() -> uint32_t {          // the next tile of the ring
       const uint32_t s = c % Sh::kStages;
-      ok = ok && mbar_wait_warp(bar(KV_FULL + s), (c / Sh::kStages) & 1, abort_flag, &g_status);
+      ok = ok && mbar_wait_warp(bar(KV_FULL + s), (c / Sh::kStages) & 1, abort_flag, p.status);
       ++c;
       return warp_uniform(s);
     };
@@ -437,7 +367,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       n = (int)warp_uniform(n); w = (int)warp_uniform(w); s = warp_uniform(s);
       const uint64_t vd = make_mn_desc(sm + Sh::kRing + s * Sh::kTileBytes, Sh::kHalfBytes);
       const uint32_t more = warp_uniform(first ? 0u : 1u);
-      ok = ok && mbar_wait_warp(bar(P_FULL + w), (w == 0 ? np0 : np1) & 1, abort_flag, &g_status);
+      ok = ok && mbar_wait_warp(bar(P_FULL + w), (w == 0 ? np0 : np1) & 1, abort_flag, p.status);
       if (!ok) return;
       tc_fence_after();
 #pragma unroll
@@ -459,12 +389,12 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       __syncwarp();
     };
     for (uint32_t i = 0; ok; ++i) {
-      if (!mbar_wait_warp(bar(ITEM_FULL + (i & 1)), (i >> 1) & 1, abort_flag, &g_status)) break;
+      if (!mbar_wait_warp(bar(ITEM_FULL + (i & 1)), (i >> 1) & 1, abort_flag, p.status)) break;
       const Item it = uniform_item(item_at(i));
       if (lane == 0) mbar_arrive(bar(ITEM_EMPTY + (i & 1)));
       if (it.last) break;
       if (it.n == 0) continue;
-      if (!mbar_wait_warp(bar(Q_FULL), nq & 1, abort_flag, &g_status)) break;
+      if (!mbar_wait_warp(bar(Q_FULL), nq & 1, abort_flag, p.status)) break;
       ++nq;
       const int most = seen(it, causal, min(it.q_left, it.dual ? 2 * tile_tokens : tile_tokens) - 1);
       if (it.dual) {
@@ -540,7 +470,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     float* const join_ml = reinterpret_cast<float*>(sp + Sh::kJoinMl) + row * 2;
     bool ok = true;
     for (uint32_t i = 0; ok; ++i) {
-      if (!mbar_wait_warp(bar(ITEM_FULL + (i & 1)), (i >> 1) & 1, abort_flag, &g_status)) break;
+      if (!mbar_wait_warp(bar(ITEM_FULL + (i & 1)), (i >> 1) & 1, abort_flag, p.status)) break;
       const Item it = uniform_item(item_at(i));
       if (lane == 0) mbar_arrive(bar(ITEM_EMPTY + (i & 1)));
       if (it.last) break;
@@ -553,7 +483,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       float m = -INFINITY, l = 0.f;          // m: the maximum that the weights are taken against
       bool first = true;
       for (int j = it.dual ? 0 : w; j < tiles; j += step) {
-        if (!mbar_wait_warp(bar(S_FULL + w), ns & 1, abort_flag, &g_status)) { ok = false; break; }
+        if (!mbar_wait_warp(bar(S_FULL + w), ns & 1, abort_flag, p.status)) { ok = false; break; }
         ++ns;
         if (live) {
           tc_fence_after();
@@ -636,7 +566,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       if (!ok) break;
       const bool any = (it.dual ? 0 : w) < tiles;
       if (any) {
-        if (!mbar_wait_warp(bar(O_FULL + w), no & 1, abort_flag, &g_status)) break;
+        if (!mbar_wait_warp(bar(O_FULL + w), no & 1, abort_flag, p.status)) break;
         ++no;
         tc_fence_after();
       }
@@ -652,7 +582,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           tmem_ld32(o_at + h * 64 + 32, o[1]);
           tmem_wait_ld(o[0]);
           tmem_wait_ld(o[1]);
-          ok = mbar_wait_warp(bar(JOIN_EMPTY + quarter), (nj & 1) ^ 1, abort_flag, &g_status);
+          ok = mbar_wait_warp(bar(JOIN_EMPTY + quarter), (nj & 1) ^ 1, abort_flag, p.status);
           if (!ok) break;
           ++nj;
           if (h == 0) *reinterpret_cast<float2*>(join_ml) = make_float2(m, l);
@@ -685,7 +615,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         }
         if (joined) {
           if ((b & 1) == 0) {
-            ok = mbar_wait_warp(bar(JOIN_FULL + quarter), nj & 1, abort_flag, &g_status);
+            ok = mbar_wait_warp(bar(JOIN_FULL + quarter), nj & 1, abort_flag, p.status);
             if (!ok) break;
             ++nj;
           }
@@ -725,7 +655,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     make_uint4(bf16_pair(f[0], f[1]), bf16_pair(f[2], f[3]), bf16_pair(f[4], f[5]), bf16_pair(f[6], f[7]));
             }
           } else {
-            float* const po = p.part_o + slot * a.dim;
+            float* const po = p.split.part_o + slot * a.dim;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               if (b * 32 + e * 4 < a.dim) *reinterpret_cast<uint4*>(po + b * 32 + e * 4) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
@@ -736,7 +666,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       if (!ok) break;
       if (valid) {
         const float le = mine > 0 ? fmaf(m, a.scale, logf(l)) : -INFINITY;
-        if (it.part >= 0) p.part_lse[slot] = le;
+        if (it.part >= 0) p.split.part_lse[slot] = le;
         else if (a.lse != nullptr) a.lse[token * a.heads + head] = le;
       }
       // a value that is not finite may have come in with a weight of zero: from keys that other rows of the tile see, or
@@ -747,7 +677,8 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       while (odd != 0) {
         const int src = __ffs(odd) - 1;
         odd &= odd - 1;
-        redo_row(p, it, __shfl_sync(0xffffffffu, token, src), __shfl_sync(0xffffffffu, head, src), __shfl_sync(0xffffffffu, mine, src));
+        redo_row(a, p.split, it.k_row, it.kv_head, it.part, __shfl_sync(0xffffffffu, token, src), __shfl_sync(0xffffffffu, head, src),
+                 __shfl_sync(0xffffffffu, mine, src), 0, DP);
       }
     }
   }
@@ -758,159 +689,42 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
-// Joins the chunks of a query: a warp per row and head.
-__global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ TmemAttnParams p) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const AttnParams& a = p.a;
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int64_t token = item / a.heads;
-  const int head = (int)(item - token * a.heads);
-  if (token >= a.tokens_q) return;
-  int lo = 0, hi = a.sequences;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu_q[mid] <= token) lo = mid; else hi = mid;
-  }
-  const Span sq = span_of(a.cu_q, lo, a.tokens_q);
-  if (token < sq.begin || token >= sq.begin + sq.length) return;
-  const Span sk = span_of(a.cu_k, lo, a.tokens_k);
-  const int chunks = (key_tiles((int)sk.length) + p.chunk - 1) / p.chunk;
-  if (chunks <= 1) return;                   // written by the attention kernel
-  const int64_t stride = a.tokens_q * a.heads, at = token * a.heads + head;
-  float m = -INFINITY;
-  for (int i = lane; i < chunks; i += 32) m = fmaxf(m, p.part_lse[i * stride + at]);
-  m = warp_max(m);
-  const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  float o[4] = {0.f, 0.f, 0.f, 0.f};
-  const int d = lane * 4;
-  for (int i = 0; i < chunks; ++i) {
-    const float le = p.part_lse[i * stride + at];
-    if (le == -INFINITY) continue;
-    const float f = exp2f((le - base) * kLog2e);
-    l += f;
-    if (d < a.dim) {
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + (i * stride + at) * a.dim + d);
-      o[0] = fmaf(v.x, f, o[0]);
-      o[1] = fmaf(v.y, f, o[1]);
-      o[2] = fmaf(v.z, f, o[2]);
-      o[3] = fmaf(v.w, f, o[3]);
-    }
-  }
-  const bool some = l != 0.f;                // a NaN is some, too
-  if (d < a.dim) {
-    const float inv = some ? 1.0f / l : 0.f;
-    *reinterpret_cast<uint2*>(a.out + token * a.out_token + head * a.out_head + d) =
-        make_uint2(bf16_pair(o[0] * inv, o[1] * inv), bf16_pair(o[2] * inv, o[3] * inv));
-  }
-  if (a.lse != nullptr && lane == 0) a.lse[at] = some ? base + logf(l) : -INFINITY;
-}
-
-int device_sms() {
-  static int sms[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  if (sms[dev] == 0) {
-    int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-    sms[dev] = n;
-  }
-  return sms[dev];
-}
-
-struct Plan {
-  int pack_log2, groups, chunk, chunks_most;
-  int64_t grid;
+struct Tiles {
+  int pack_log2, groups;
+  int64_t items, per_sequence;
 };
-
-// How a call is cut up.  Only its sizes are known here, not its offsets.
-Plan plan_of(const AttnParams& a, int sms) {
-  Plan plan = {};
+Tiles tiles_of(const AttnParams& a) {
+  Tiles t = {};
   const int group = a.heads / a.kv_heads;
-  while (plan.pack_log2 < 7 && group % (2 << plan.pack_log2) == 0) ++plan.pack_log2;
-  plan.groups = a.heads >> plan.pack_log2;
-  const int64_t pair_tokens = 2 * (kTile >> plan.pack_log2);
+  while (t.pack_log2 < 7 && group % (2 << t.pack_log2) == 0) ++t.pack_log2;
+  t.groups = a.heads >> t.pack_log2;
+  const int64_t pair_tokens = 2 * (kTile >> t.pack_log2);
   const int64_t pairs = a.tokens_q / pair_tokens + (a.tokens_q < a.sequences ? a.tokens_q : a.sequences);   // at most
-  const int64_t items = pairs * plan.groups;
-  const int64_t tiles = (a.tokens_k + kTile - 1) / kTile;                   // of the longest sequence there can be
-  plan.chunk = (int)(tiles < 1 ? 1 : tiles);
-  plan.chunks_most = 1;
-  if (items < 4 * (int64_t)sms) {
-    // a quarter of a CTA's share each, if the sequences are alike; no fewer than 4 tiles, which a chunk's start would outweigh
-    int64_t chunk = (tiles + a.sequences) * plan.groups * ((pairs + a.sequences - 1) / a.sequences) / (4 * (int64_t)sms);
-    if (chunk < 4) chunk = 4;
-    const int64_t most_bytes = 256ll << 20, row = a.tokens_q * a.heads * (a.dim + 1) * 4;
-    while (chunk < tiles && (tiles + chunk - 1) / chunk * row > most_bytes) chunk *= 2;
-    if (chunk < tiles) {
-      plan.chunk = (int)chunk;
-      plan.chunks_most = (int)((tiles + chunk - 1) / chunk);
-    }
-  }
-  const int64_t most = items * plan.chunks_most;
-  plan.grid = most < sms ? most : sms;
-  return plan;
-}
-
-int64_t part_lse_offset(const AttnParams& a, const Plan& plan) {
-  return ((int64_t)plan.chunks_most * a.tokens_q * a.heads * a.dim * 4 + 255) / 256 * 256;
-}
-
-bool strides_for_tma(int64_t token, int64_t head, int heads, int64_t tokens) {
-  auto fine = [](int64_t s, int64_t n) { return n == 1 || (s > 0 && s % 8 == 0 && s < (1ll << 38)); };
-  return fine(head, heads) && fine(token, tokens);
+  t.items = pairs * t.groups;
+  t.per_sequence = (pairs + a.sequences - 1) / a.sequences * t.groups;
+  return t;
 }
 
 }  // namespace
 
-bool attention_tmem_supported(const AttnParams& a) {
-  auto al = [](const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
-  return a.dim <= 128 && a.dim % 8 == 0 && a.tokens_k > 0 && al(a.q, 16) && al(a.k, 16) && al(a.v, 16) && al(a.out, 16) &&
-         a.out_token % 8 == 0 && a.out_head % 8 == 0 && strides_for_tma(a.q_token, a.q_head, a.heads, a.tokens_q) &&
-         strides_for_tma(a.k_token, a.k_head, a.kv_heads, a.tokens_k) && strides_for_tma(a.v_token, a.v_head, a.kv_heads, a.tokens_k);
+AttnSplit attention_tmem_split(const AttnParams& a, void* workspace) {
+  const Tiles t = tiles_of(a);
+  return attention_split(a, t.items, t.per_sequence, device_sms(), 4, workspace);
 }
 
-int64_t attention_tmem_workspace(const AttnParams& a) {
-  const Plan plan = plan_of(a, device_sms());
-  return plan.chunks_most == 1 ? 0 : part_lse_offset(a, plan) + (int64_t)plan.chunks_most * a.tokens_q * a.heads * 4;
-}
-
-int attention_tmem_status(int* out) {
-  SACQ_CUDA_TRY(cudaMemcpyFromSymbol(out, g_status, sizeof(int)));
-  return SACQ_OK;
-}
-
-int launch_attention_tmem(const AttnParams& a, void* workspace, int64_t workspace_bytes, cudaStream_t s) {
-  const Plan plan = plan_of(a, device_sms());
+int launch_attention_tmem(const AttnParams& a, const AttnSplit& split, cudaStream_t s) {
+  const Tiles t = tiles_of(a);
   TmemAttnParams p = {};
   p.a = a;
-  p.pack_log2 = plan.pack_log2;
-  p.groups = plan.groups;
-  p.chunk = plan.chunk;
-  p.chunks_most = plan.chunks_most;
-  if (plan.chunks_most > 1) {
-    const int64_t need = attention_tmem_workspace(a);
-    if (workspace == nullptr || workspace_bytes < need)
-      return set_error(SACQ_ERR_WORKSPACE, "workspace of %lld bytes, %lld are needed", (long long)(workspace ? workspace_bytes : 0), (long long)need);
-    if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return set_error(SACQ_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
-    p.part_o = static_cast<float*>(workspace);
-    p.part_lse = reinterpret_cast<float*>(static_cast<char*>(workspace) + part_lse_offset(a, plan));
-  }
-  // the stride of a dimension of one element means nothing, but is checked
-  auto stride = [](int64_t s, int64_t n, int64_t other) { return n == 1 ? other : s; };
+  p.pack_log2 = t.pack_log2;
+  p.groups = t.groups;
+  p.split = split;
+  p.status = attention_status_word();
+  if (p.status == nullptr) return set_error(SACQ_ERR_CUDA, "no status word on this device");
+  const int64_t most = t.items * split.chunks_most;
   CUtensorMap mq, mk, mv;
-  const int pack = 1 << plan.pack_log2;
-  const int64_t dim8 = a.dim;
-  auto make = [&](CUtensorMap* m, const void* base, int64_t tokens, int heads, int64_t token, int64_t head, int box_heads, int box_tokens) {
-    const int64_t h = stride(head, heads, dim8), t = stride(token, tokens, dim8 * heads);
-    return encode_bf16_3d(m, base, (uint64_t)a.dim, (uint64_t)heads, (uint64_t)tokens, (uint64_t)h, (uint64_t)t, 64u, (uint32_t)box_heads, (uint32_t)box_tokens,
-                          CU_TENSOR_MAP_SWIZZLE_128B);
-  };
-  int rc = make(&mq, a.q, a.tokens_q, a.heads, a.q_token, a.q_head, pack, kTile / pack);
-  if (rc == SACQ_OK) rc = make(&mk, a.k, a.tokens_k, a.kv_heads, a.k_token, a.k_head, 1, kTile);
-  if (rc == SACQ_OK) rc = make(&mv, a.v, a.tokens_k, a.kv_heads, a.v_token, a.v_head, 1, kTile);
-  if (rc != SACQ_OK) return rc;
+  const int pack = 1 << t.pack_log2;
+  if (int rc = attention_tensor_maps(a, pack, kTile / pack, kTile, &mq, &mk, &mv)) return rc;
   const bool wide = a.dim > 64;
   const void* fn = wide ? (const void*)attention_tmem_kernel<128> : (const void*)attention_tmem_kernel<64>;
   const size_t smem = (wide ? Shape<128>::kTotal : Shape<64>::kTotal) + 1024;
@@ -922,7 +736,7 @@ int launch_attention_tmem(const AttnParams& a, void* workspace, int64_t workspac
     if (dev >= 0 && dev < 64) configured[wide][dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)plan.grid);
+  cfg.gridDim = dim3((unsigned)(most < device_sms() ? most : device_sms()));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -934,15 +748,6 @@ int launch_attention_tmem(const AttnParams& a, void* workspace, int64_t workspac
   void* args[] = {&mq, &mk, &mv, &p};
   SACQ_CUDA_TRY(cudaLaunchKernelExC(&cfg, fn, args));
   count_launch();
-  if (plan.chunks_most > 1) {
-    const int64_t grid = (a.tokens_q * a.heads + 3) / 4;
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(128);
-    cfg.dynamicSmemBytes = 0;
-    void* join_args[] = {&p};
-    SACQ_CUDA_TRY(cudaLaunchKernelExC(&cfg, (const void*)attention_join_kernel, join_args));
-    count_launch();
-  }
   return SACQ_OK;
 }
 

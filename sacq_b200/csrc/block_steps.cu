@@ -116,11 +116,27 @@ AttnParams attention_params(const sacq_attention_desc* d) {
 
 }  // namespace
 
+namespace {
+
+enum { kByRows, kShort, kTmem };
+// Sequences of few rows (queries x heads of a group) are bound by reading their keys: a kernel of 16-row tiles for them.  Only the
+// average is known here.
+int attention_kernel(const AttnParams& p) {
+  if (!attention_tma_supported(p)) return kByRows;
+  return p.tokens_q * (p.heads / p.kv_heads) <= 32 * (int64_t)p.sequences ? kShort : kTmem;
+}
+AttnSplit split_for(const AttnParams& p, int kernel, void* workspace) {
+  return kernel == kShort ? attention_short_split(p, workspace) : attention_tmem_split(p, workspace);
+}
+
+}  // namespace
+
 SACQ_API int64_t sacq_attention_workspace_bytes(const sacq_attention_desc* d) {
   if (int rc = check_attention(d)) return rc;
   if (d->tokens_q == 0 || d->sequences == 0) return 0;
   const AttnParams p = attention_params(d);
-  return attention_tmem_supported(p) ? attention_tmem_workspace(p) : 0;
+  const int kernel = attention_kernel(p);
+  return kernel == kByRows ? 0 : attention_split_bytes(p, split_for(p, kernel, nullptr));
 }
 
 SACQ_API int sacq_attention_packed(const sacq_attention_desc* d, void* stream) {
@@ -130,14 +146,24 @@ SACQ_API int sacq_attention_packed(const sacq_attention_desc* d, void* stream) {
       (d->tokens_k > 0 && (d->k == nullptr || d->v == nullptr)))
     return set_error(SACQ_ERR_INVALID_ARGUMENT, "null argument");
   const AttnParams p = attention_params(d);
-  if (attention_tmem_supported(p)) return launch_attention_tmem(p, d->workspace, d->workspace_bytes, static_cast<cudaStream_t>(stream));
-  return launch_attention_rows(p, static_cast<cudaStream_t>(stream));
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int kernel = attention_kernel(p);
+  if (kernel == kByRows) return launch_attention_rows(p, s);
+  const AttnSplit split = split_for(p, kernel, d->workspace);
+  const int64_t need = attention_split_bytes(p, split);
+  if (need > 0) {
+    if (d->workspace == nullptr || d->workspace_bytes < need)
+      return set_error(SACQ_ERR_WORKSPACE, "workspace of %lld bytes, %lld are needed", (long long)(d->workspace ? d->workspace_bytes : 0), (long long)need);
+    if (reinterpret_cast<uintptr_t>(d->workspace) % 256 != 0) return set_error(SACQ_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
+  }
+  if (int rc = kernel == kShort ? launch_attention_short(p, split, s) : launch_attention_tmem(p, split, s)) return rc;
+  return split.chunks_most > 1 ? launch_attention_join(p, split, s) : SACQ_OK;
 }
 
 SACQ_API int sacq_block_steps_status(int* status_out) {
   if (status_out == nullptr) return set_error(SACQ_ERR_INVALID_ARGUMENT, "null argument");
   int norm = 0;
-  if (int rc = attention_tmem_status(status_out)) return rc;
+  if (int rc = attention_status(status_out)) return rc;
   if (int rc = residual_norm_status(&norm)) return rc;
   *status_out |= norm;
   return SACQ_OK;
