@@ -40,9 +40,10 @@ struct TmemAttnParams {
   int groups;                               // heads / pack
   AttnSplit split;
   int* status;
+  int dynamic;                              // a CTA per item that there can be: running CTAs take over those that have not begun
 };
 
-struct Item {
+struct alignas(16) Item {
   int last;                                 // no more items
   int q_row, q_left;                        // first query row; rows of the sequence from it on
   int head, kv_head;
@@ -72,7 +73,7 @@ struct Shape {
 };
 // mbarriers
 constexpr int Q_FULL = 0, Q_EMPTY = 1, S_FULL = 2, P_FULL = 4, O_FULL = 6, ITEM_FULL = 10, ITEM_EMPTY = 12,
-              DRAIN = 14, KV_FULL = 16, KV_EMPTY = 32, JOIN_FULL = 48, JOIN_EMPTY = 52;
+              DRAIN = 14, TAKE = 15, KV_FULL = 16, KV_EMPTY = 32, JOIN_FULL = 48, JOIN_EMPTY = 52;
 
 __device__ __forceinline__ void umma_bf16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -153,6 +154,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float log2_fast(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // The largest of three, NaN if one is.
 __device__ __forceinline__ float max_nan(float a, float b, float c) {
   float r;
@@ -185,6 +191,22 @@ __device__ __forceinline__ uint64_t exp2_polynomial(uint64_t v) {
   halves_of(r, a, b);
   halves_of(t, ta, tb);
   return f32x2(__uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23)), __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23)));
+}
+// Asks for a CTA of the grid that has not begun; it will not, and the answer (16 bytes) says which it was, or that there was none.
+__device__ __forceinline__ void request_cta(uint32_t answer, uint32_t bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+__device__ __forceinline__ bool answered_cta(uint32_t answer, uint32_t& cta) {
+  uint32_t yes, x;
+  asm volatile(
+      "{\n\t.reg .b128 a;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 a, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, a;\n\t}"
+      : "=r"(yes), "=r"(x) : "r"(answer) : "memory");
+  cta = x;
+  return yes != 0;
 }
 // An item's fields, the same in all lanes and known to be: what is computed from them may stay in uniform registers.
 __device__ __forceinline__ Item uniform_item(const Item* at) {
@@ -232,6 +254,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       mbar_init(bar(ITEM_EMPTY + w), 9);
     }
     mbar_init(bar(DRAIN), 1);
+    mbar_init(bar(TAKE), 1);
     for (int i = 0; i < 4; ++i) {
       mbar_init(bar(JOIN_FULL + i), 1);
       mbar_init(bar(JOIN_EMPTY + i), 1);
@@ -277,11 +300,37 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     };
     ItemList<decltype(count)> list{a, count};
     list.look();
-    for (int64_t index = blockIdx.x; ok; index += gridDim.x) {
+    // the next item: the CTA's stride further, or one that is taken over; asked for while this one's copies are issued
+    const uint32_t answer = sm + Sh::kMisc + 16;
+    uint32_t taken = 0;
+    bool more = true;
+    auto ask = [&] {
+      if (p.dynamic && elect_one()) {
+        fence_proxy_async();
+        mbar_arrive_expect_tx(bar(TAKE), 16);
+        request_cta(answer, bar(TAKE));
+      }
+      __syncwarp();
+    };
+    auto advance = [&](int64_t& index) {
+      if (!p.dynamic) {
+        index += gridDim.x;
+        return;
+      }
+      ok = mbar_wait_warp(bar(TAKE), taken & 1, abort_flag, p.status);
+      ++taken;
+      uint32_t cta = 0;
+      more = ok && answered_cta(answer, cta);
+      index = cta;
+      __syncwarp();
+    };
+    for (int64_t index = blockIdx.x; ok; advance(index)) {
       Item it = {};
       Span sq, sk;
       int64_t r;
-      it.last = !list.find(index, sq, sk, r);
+      it.last = !more || !list.find(index, sq, sk, r);
+      if (more) ask();
+      if (p.dynamic && more && it.last) continue;            // there can be more items than there are: their CTAs need not begin
       if (!it.last) {
         // heads first, then chunks; the pairs of tiles from the last, longest one to the first
         const int lq = (int)sq.length, lk = (int)sk.length, chunks = chunks_of(p.split, lk);
@@ -331,7 +380,9 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         if (j + ahead < it.n) take(&map_k, it, j + ahead);
       }
     }
-    if (*abort_flag)                         // copies in flight land before the CTA leaves
+    if (*abort_flag && p.dynamic)            // what is in flight lands before the CTA leaves
+      for (int t = 0; t < 100000 && !mbar_try_wait(bar(TAKE), taken & 1); ++t) {}
+    if (*abort_flag)
       for (uint32_t i = c > Sh::kStages ? c - Sh::kStages : 0; i < c; ++i)
         for (int t = 0; t < 100000 && !mbar_try_wait(bar(KV_FULL + i % Sh::kStages), (i / Sh::kStages) & 1); ++t) {}
   } else if (warp == kMmaWarp) {
@@ -471,7 +522,9 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     bool ok = true;
     for (uint32_t i = 0; ok; ++i) {
       if (!mbar_wait_warp(bar(ITEM_FULL + (i & 1)), (i >> 1) & 1, abort_flag, p.status)) break;
-      const Item it = uniform_item(item_at(i));
+      Item it = *item_at(i);
+      it.last = (int)warp_uniform(it.last); it.n = (int)warp_uniform(it.n); it.n0 = (int)warp_uniform(it.n0);
+      it.dual = (int)warp_uniform(it.dual); it.part = (int)warp_uniform(it.part);
       if (lane == 0) mbar_arrive(bar(ITEM_EMPTY + (i & 1)));
       if (it.last) break;
       const int t = (row >> p.pack_log2) + (it.dual ? w * tile_tokens : 0);      // token of the item
@@ -599,27 +652,29 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       }
       const int64_t token = (int64_t)it.q_row + t;
       const int head = it.head + (row & ((1 << p.pack_log2) - 1));
-      uint16_t* const out = a.out + token * a.out_token + head * a.out_head;
       const int64_t slot = ((int64_t)max(it.part, 0) * a.tokens_q + token) * a.heads + head;
+      // rows leave through shared memory, 128 bytes of each at a time, so that a store covers 4 rows' lines and not 32
+      uint8_t* const stage = sp + Sh::kJoin + quarter * 8192 + w * 4096;
+      if (w == 1 && !mbar_wait_warp(bar(JOIN_EMPTY + quarter), (nj & 1) ^ 1, abort_flag, p.status)) break;      // its own sums have been read
       float inv = 0.f, scale0 = 1.f, scale1 = 0.f;
       bool finite = true;
 #pragma unroll 1
-      for (int b = 0; b < DP / 32; ++b) {
-        uint32_t o[32];
+      for (int h = 0; h < Sh::kHalves; ++h) {
+        uint32_t o[2][32];
         if (any) {
-          tmem_ld32(o_at + b * 32, o);
-          tmem_wait_ld(o);
+          tmem_ld32(o_at + h * 64, o[0]);
+          tmem_ld32(o_at + h * 64 + 32, o[1]);
+          tmem_wait_ld(o[0]);
+          tmem_wait_ld(o[1]);
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
+          for (int e = 0; e < 64; ++e) o[e >> 5][e & 31] = 0u;
         }
         if (joined) {
-          if ((b & 1) == 0) {
-            ok = mbar_wait_warp(bar(JOIN_FULL + quarter), nj & 1, abort_flag, p.status);
-            if (!ok) break;
-            ++nj;
-          }
-          if (b == 0) {
+          ok = mbar_wait_warp(bar(JOIN_FULL + quarter), nj & 1, abort_flag, p.status);
+          if (!ok) break;
+          ++nj;
+          if (h == 0) {
             const float2 ml = *reinterpret_cast<const float2*>(join_ml);
             const float high = fmaxf(m, ml.x);
             scale0 = m == -INFINITY ? 0.f : exp2_fast((m - high) * c2);
@@ -628,52 +683,79 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             m = high;
           }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint4 v = *reinterpret_cast<const uint4*>(join + ((((b & 1) * 8 + e) ^ (row & 15)) << 2));
-            const uint32_t* u = &v.x;
+          for (int e = 0; e < 16; ++e) {
+            const uint4 v = *reinterpret_cast<const uint4*>(join + ((e ^ (row & 15)) << 2));
+            const uint32_t* const u = &v.x;
 #pragma unroll
-            for (int f = 0; f < 4; ++f)
-              o[4 * e + f] = __float_as_uint(fmaf(__uint_as_float(u[f]), scale1, __uint_as_float(o[4 * e + f]) * scale0));
+            for (int f = 0; f < 4; ++f) {
+              uint32_t& x = o[e >> 3][4 * (e & 7) + f];
+              x = __float_as_uint(fmaf(__uint_as_float(u[f]), scale1, __uint_as_float(x) * scale0));
+            }
           }
           __syncwarp();
-          if ((b & 1) && lane == 0) mbar_arrive(bar(JOIN_EMPTY + quarter));
         }
-        if (b == 0) inv = mine > 0 ? 1.0f / l : 0.f;
-        if (valid) {
+        if (h == 0) inv = mine > 0 ? 1.0f / l : 0.f;
+        const uint64_t inv2 = f32x2(inv, inv);
+        uint64_t odd2 = f32x2(0.f, 0.f);     // NaN if a value is not finite
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float x = mine > 0 ? __uint_as_float(o[e]) * inv : 0.f;
-            finite = finite && fabsf(x) < INFINITY;
-            o[e] = __float_as_uint(x);
+        for (int e = 0; e < 32; ++e) {
+          uint32_t* const u = &o[e >> 4][2 * (e & 15)];
+          const uint64_t v = mul2(f32x2(__uint_as_float(u[0]), __uint_as_float(u[1])), inv2);
+          odd2 = fma2(v, f32x2(0.f, 0.f), odd2);
+          float x, y;
+          halves_of(v, x, y);
+          u[0] = __float_as_uint(x);
+          u[1] = __float_as_uint(y);
+        }
+        float odd0, odd1;
+        halves_of(odd2, odd0, odd1);
+        if (mine > 0) {
+          finite = finite && odd0 + odd1 == 0.f;
+        } else {                             // a row that sees nothing: zeros, whatever was multiplied by none of its weights
+#pragma unroll
+          for (int e = 0; e < 64; ++e) o[e >> 5][e & 31] = 0u;
+        }
+        if (it.part < 0) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float* const f = reinterpret_cast<const float*>(&o[e >> 2][8 * (e & 3)]);
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+                make_uint4(bf16_pair(f[0], f[1]), bf16_pair(f[2], f[3]), bf16_pair(f[4], f[5]), bf16_pair(f[6], f[7]));
           }
-          if (it.part < 0) {
+          __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float* f = reinterpret_cast<const float*>(&o[8 * e]);
-              if (b * 32 + e * 8 < a.dim)
-                *reinterpret_cast<uint4*>(out + b * 32 + e * 8) =
-                    make_uint4(bf16_pair(f[0], f[1]), bf16_pair(f[2], f[3]), bf16_pair(f[4], f[5]), bf16_pair(f[6], f[7]));
-            }
-          } else {
-            float* const po = p.split.part_o + slot * a.dim;
+          for (int e = 0; e < 8; ++e) {
+            const int r = e * 4 + (lane >> 3), piece = lane & 7, rr = quarter * 32 + r;
+            const int tt = (rr >> p.pack_log2) + (it.dual ? w * tile_tokens : 0), d = h * 64 + piece * 8;
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((piece ^ (r & 7)) << 4));
+            if (tt < it.q_left && d < a.dim)
+              *reinterpret_cast<uint4*>(a.out + ((int64_t)it.q_row + tt) * a.out_token + (int64_t)(it.head + (rr & ((1 << p.pack_log2) - 1))) * a.out_head + d) = v;
+          }
+        } else if (valid) {
+          float* const po = p.split.part_o + slot * a.dim + h * 64;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (b * 32 + e * 4 < a.dim) *reinterpret_cast<uint4*>(po + b * 32 + e * 4) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          for (int e = 0; e < 16; ++e) {
+            const uint32_t* const u = &o[e >> 3][4 * (e & 7)];
+            if (h * 64 + e * 4 < a.dim) *reinterpret_cast<uint4*>(po + e * 4) = make_uint4(u[0], u[1], u[2], u[3]);
           }
         }
         __syncwarp();
+        if (joined && lane == 0) mbar_arrive(bar(JOIN_EMPTY + quarter));
       }
       if (!ok) break;
       if (valid) {
-        const float le = mine > 0 ? fmaf(m, a.scale, logf(l)) : -INFINITY;
+        const float le = mine > 0 ? fmaf(m, a.scale, log2_fast(l) * 0.693147180559945f) : -INFINITY;
         if (it.part >= 0) p.split.part_lse[slot] = le;
         else if (a.lse != nullptr) a.lse[token * a.heads + head] = le;
       }
       // a value that is not finite may have come in with a weight of zero: from keys that other rows of the tile see, or
       // that share an instruction with them
-      const int most = seen(it, causal, min(it.q_left, (it.dual && w == 1 ? 2 : 1) * tile_tokens) - 1);
       __syncwarp();                          // the rows as they are lie in front of the ones made again
-      uint32_t odd = __ballot_sync(0xffffffffu, valid && !finite && mine > 0 && mine < min((most + 15) & ~15, it.keys));
+      uint32_t odd = __ballot_sync(0xffffffffu, valid && !finite);
+      if (odd != 0) {
+        const int most = seen(it, causal, min(it.q_left, (it.dual && w == 1 ? 2 : 1) * tile_tokens) - 1);
+        odd = __ballot_sync(0xffffffffu, valid && !finite && mine < min((most + 15) & ~15, it.keys));
+      }
       while (odd != 0) {
         const int src = __ffs(odd) - 1;
         odd &= odd - 1;
@@ -736,7 +818,10 @@ int launch_attention_tmem(const AttnParams& a, const AttnSplit& split, cudaStrea
     if (dev >= 0 && dev < 64) configured[wide][dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(most < device_sms() ? most : device_sms()));
+  // Items differ in length (a causal prompt's last tile has all its keys): CTAs that take the next one when they are done
+  // end together (two prompts of 8192 and 6001: 412 against 446 us).  Not with chunks, of which there can be many more than there are.
+  p.dynamic = split.chunks_most == 1 && most > device_sms() && most <= 2147483647;
+  cfg.gridDim = dim3((unsigned)(p.dynamic || most < device_sms() ? most : device_sms()));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
