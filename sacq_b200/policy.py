@@ -17,14 +17,20 @@ adds run inside this library's quantizer and GEMM kernels; every projection is a
 ``PrecomputedPackedVectorCodebookLinear`` (dim-8 vectors, 4096-entry codebook,
 per-output-channel scales).  The cross-attention keys/values depend only on the language
 tokens and are computed once per query, not once per denoising step.
+
+``forward`` takes requests of equal length.  ``forward_packed`` takes requests whose prompts differ in length, one behind the other
+without padding, and runs on this library alone: attention over packed sequences, a causal language model with rotary
+positions, gated branches in the action head, and residual adds inside the next norm's kernel.
 """
 from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
 
-from .activation import act_quantize_rows, layernorm_quantize_rows, quantize_rows
+from .activation import act_quantize_rows, layernorm_quantize_rows, quantize_rows, residual_norm_quantize_rows
+from .attention import attention_packed
 from .linear import PrecomputedPackedVectorCodebookLinear, forward_shared, linear_a8_multi
+from .rotary import rotary_frequencies, rotate_heads
 from .synthetic import make_payload
 
 
@@ -114,6 +120,35 @@ class _Block(torch.nn.Module):
             qd, sd = act_quantize_rows("gelu", self.up.linear_a8(qu, su))
         return self.down.linear_a8(qd, sd, residual=x)
 
+    def _add_norm(self, norm, branch, x, gate=None, scale=None, shift=None):
+        """x + gate * branch and its LayerNorm (+ AdaLN modulation) as the next projections' 8-bit rows, in one launch."""
+        return residual_norm_quantize_rows(branch, x, norm.weight, norm.bias, norm="layer", eps=norm.eps, gate=gate, mod_scale=scale,
+                                           mod_shift=shift)
+
+    def forward_packed(self, x, cu, causal=False, rotary=None, cross=None, modulation=None, gates=None):
+        """The block on packed rows.  cu: offsets of the sequences; rotary: (positions, inv_freq) of a language model's heads;
+        cross: (keys, values, offsets) of the context; gates: vectors of the self- and the cross-attention's branch."""
+        t = x.shape[0]
+        m = (None,) * 4 if modulation is None else modulation.view(4, self.hidden)
+        gates = (None, None) if gates is None else gates
+        qa, sa = self._norm_quant(self.n1, x, m[1], m[0])
+        q, k, v = (y.view(t, -1, self.head_dim) for y in linear_a8_multi((self.q, self.k, self.v), qa, sa))
+        if rotary is not None:
+            rotate_heads(q, k, *rotary, out=(q, k))
+        branch, gate = self.o(attention_packed(q, k, v, cu, causal=causal).view(t, self.hidden)), gates[0]
+        if self.cross:
+            x, qc, sc = self._add_norm(self.n3, branch, x, gate)
+            ck, cv, cu_k = cross
+            a = attention_packed(self.cq.linear_a8(qc, sc).view(t, -1, self.head_dim), ck.view(ck.shape[0], -1, self.head_dim),
+                                 cv.view(cv.shape[0], -1, self.head_dim), cu, cu_k)
+            branch, gate = self.co(a.view(t, self.hidden)), gates[1]
+        x, qu, su = self._add_norm(self.n2, branch, x, gate, m[3], m[2])
+        if self.gated:
+            qd, sd = act_quantize_rows("silu_mul", *linear_a8_multi((self.gate, self.up), qu, su))
+        else:
+            qd, sd = act_quantize_rows("gelu", self.up.linear_a8(qu, su))
+        return self.down.linear_a8(qd, sd, residual=x)
+
 
 class SyntheticGr00tPolicy(torch.nn.Module):
     VIT_LAYERS, VIT_HIDDEN, VIT_MLP, PATCHES = 24, 1024, 4096, 256
@@ -142,6 +177,9 @@ class SyntheticGr00tPolicy(torch.nn.Module):
         self.action_out = (torch.randn(self.DIT_HIDDEN, self.ACTION_DIM, generator=g) * 0.02).to(**bf)
         self.num_quantized_linears = f.count
         self.device = dev
+        # of the packed forward: gates of the action head's attention branches, frequencies of the language model's heads
+        self.dit_gates = (1 + torch.randn(self.DIT_LAYERS, 2, self.DIT_HIDDEN, generator=g) * 0.1).to(**bf)
+        self.llm_inv_freq = rotary_frequencies(self.LLM_HIDDEN // 16, base=1e6, device=dev)[0]
 
     def quantized_linear_calls_per_query(self) -> int:
         vit = self.VIT_LAYERS * 6
@@ -187,6 +225,49 @@ class SyntheticGr00tPolicy(torch.nn.Module):
             actions = actions + dt * (h @ self.action_out)
         actions = actions.view(b, self.HORIZON, self.ACTION_DIM)
         return actions[0] if single else actions
+
+    @torch.no_grad()
+    def forward_packed(self, image: torch.Tensor, noise: torch.Tensor, prompt_lengths) -> torch.Tensor:
+        """image [B, 3, 224, 224] and noise [B, HORIZON, ACTION_DIM] of B requests whose prompts have ``prompt_lengths`` (a
+        sequence of B integers from 0 to LLM_TOKENS - PATCHES) text tokens behind the image's -> actions [B, HORIZON, ACTION_DIM].
+        Requests lie one behind the other in every linear and in attention; none is padded.  A workload of its own, not
+        ``forward``'s numbers: the language model is causal and has rotary positions, the action head's attention branches
+        are gated."""
+        lengths = [int(n) for n in prompt_lengths]
+        b = image.shape[0]
+        if len(lengths) != b or noise.shape[0] != b:
+            raise ValueError("image, noise and prompt_lengths must have one entry per request")
+        if any(not 0 <= n <= self.LLM_TOKENS - self.PATCHES for n in lengths):
+            raise ValueError(f"a prompt has 0 to {self.LLM_TOKENS - self.PATCHES} text tokens")
+
+        def offsets(counts):
+            return torch.tensor([0, *counts], dtype=torch.int32).cumsum(0, dtype=torch.int32).to(self.device)
+
+        cu_image, cu_action = offsets([self.PATCHES] * b), offsets([self.HORIZON] * b)
+        total = [self.PATCHES + n for n in lengths]
+        cu_text = offsets(total)
+        positions = torch.cat([torch.arange(n, dtype=torch.int32) for n in total]).to(self.device)
+        patches = image.unfold(2, 14, 14).unfold(3, 14, 14).permute(0, 2, 3, 1, 4, 5).reshape(b * self.PATCHES, -1)
+        x = patches @ self.patch_embed
+        for blk in self.vit:
+            x = blk.forward_packed(x, cu_image)
+        vis = self.vis_proj(x).view(b, self.PATCHES, self.LLM_HIDDEN)
+        tokens = torch.cat([t for i, n in enumerate(lengths) for t in (vis[i], self.text_embed[:n])])
+        for blk in self.llm:
+            tokens = blk.forward_packed(tokens, cu_text, causal=True, rotary=(positions, self.llm_inv_freq))
+        kv = [(*blk.cross_kv(tokens), cu_text) for blk in self.dit]
+        actions = noise.reshape(b * self.HORIZON, self.ACTION_DIM)
+        dt = 1.0 / self.STEPS
+        for step in range(self.STEPS):
+            qc, sc = quantize_rows(self.time_embed[step: step + 1])
+            mods = []
+            for i in range(0, len(self.dit), 4):
+                mods += linear_a8_multi([blk.mod for blk in self.dit[i: i + 4]], qc, sc)
+            h = actions @ self.action_in
+            for blk, cross, mod, gates in zip(self.dit, kv, mods, self.dit_gates):
+                h = blk.forward_packed(h, cu_action, cross=cross, modulation=mod, gates=gates)
+            actions = actions + dt * (h @ self.action_out)
+        return actions.view(b, self.HORIZON, self.ACTION_DIM)
 
     def example_inputs(self, seed: int = 42, batch: int = 1):
         """Seeded inputs: one request ([3, 224, 224], [HORIZON, ACTION_DIM]) for batch = 1, else

@@ -264,15 +264,17 @@ def _rotary_reference(x, positions, inv_freq, layout, amplitude):
     y, tol = x.clone(), torch.zeros_like(x)
     a, b = x[..., first], x[..., second]
     y[..., first], y[..., second] = a * c - b * s, b * c + a * s
-    # the angle rounded to 2^-26 turns (2^-23.3 radians), sine and cosine to 2 ulp, three fp32 operations; the result to bf16
-    small = (a.abs() + b.abs()) * abs(amplitude) * 2.0 ** -20
+    # the angle rounded to 2^-26 turns (2^-23.3 radians), sine and cosine to 2 ulp, three fp32 operations; the result to bf16.  In double the
+    # kernel rounds inv_freq / 2 pi and its product with the position, this reference its own product: 3 x 2^-53 of the angle, which at
+    # 2^33 positions is 2.9e-6 radians and more than all the rest
+    small = (a.abs() + b.abs()) * abs(amplitude) * (2.0 ** -20 + angle.abs() * 3 * 2.0 ** -53)
     tol[..., first] = tol[..., second] = small
     return y, torch.where(tol > 0, tol * 1.01 + y.abs() * BF, 0.0)
 
 
 @pytest.mark.parametrize("layout", ("half", "interleaved"))
 @pytest.mark.parametrize("tokens,heads,kv_heads,dim,rotary", ((1, 16, 8, 128, 128), (3, 12, 12, 128, 64), (257, 6, 2, 96, 96), (1000, 4, 4, 80, 40), (37, 1, 1, 64, 2),
-                                                              (5, 2, 1, 36, 20), (64, 3, 3, 7, 6), (19, 128, 1, 64, 64), (2, 2, 2, 512, 256), (700, 32, 8, 128, 32)))
+                                                              (5, 2, 1, 36, 20), (64, 3, 3, 7, 6), (19, 128, 1, 64, 64), (2, 2, 2, 512, 256), (700, 32, 8, 128, 32), (800, 1, 1, 4096, 4096)))
 def test_rotary(layout, tokens, heads, kv_heads, dim, rotary):
     from sacq_b200 import rotary_frequencies, rotate_heads
     gen = _gen(tokens)
@@ -555,3 +557,83 @@ def test_steps_follow_the_kernel_in_front():
             big = big @ big * 1e-3
         y.add_(x, alpha=0.5)
         assert _same(_steps(y, inputs), want)
+
+
+def test_policy_of_prompts_of_different_lengths():
+    """The packed forward gives each request what it gets alone, up to the roundings that other kernels of the linears bring
+    (the bar of the batched policy: 2e-2 relative), and requests do not reach each other."""
+    from sacq_b200.policy import SyntheticGr00tPolicy
+    policy = SyntheticGr00tPolicy("cuda", seed=3)
+    image, noise = policy.example_inputs(9, batch=3)
+    lengths = [44, 0, 17]
+    got = policy.forward_packed(image, noise, lengths)
+    assert tuple(got.shape) == (3, 16, 32) and bool(torch.isfinite(got.float()).all())
+    assert torch.equal(got, policy.forward_packed(image, noise, lengths))
+    for i in range(3):
+        one = policy.forward_packed(image[i:i + 1], noise[i:i + 1], lengths[i:i + 1])[0]
+        err = ((got[i].float() - one.float()).norm() / one.float().norm()).item()
+        assert err <= 2e-2, (i, err)
+    other = image.clone()
+    other[1] = 1.0 - other[1]
+    again = policy.forward_packed(other, noise, lengths)
+    assert torch.equal(again[0], got[0]) and torch.equal(again[2], got[2]) and not torch.equal(again[1], got[1])
+    for bad in ([44, 0], [44, 0, 45], [-1, 0, 1]):
+        with pytest.raises(ValueError):
+            policy.forward_packed(image, noise, bad)
+
+
+def test_steps_refuse_what_they_cannot_do():
+    from sacq_b200 import attention_packed, residual_norm_quantize_rows, rotary_frequencies, rotate_heads
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    q, k, cu = z(4, 4, 64), z(4, 2, 64), _offsets([4])
+    for args in ((q, k, z(5, 2, 64), cu), (q, z(4, 3, 64), z(4, 3, 64), cu), (q, z(4, 2, 32), z(4, 2, 32), cu), (z(4, 4, 264), z(4, 2, 264), z(4, 2, 264), cu),
+                 (q, k, k, cu, _offsets([2, 2])), (q, k, k, cu.cpu())):
+        with pytest.raises(ValueError):
+            attention_packed(*args)
+    for args in ((q, k, k, cu.long()), (q, k, k, cu.view(1, -1)), (q.float(), k, k, cu)):
+        with pytest.raises(TypeError):
+            attention_packed(*args)
+    for scale in (0.0, -1.0, INF, NAN):
+        with pytest.raises(ValueError):
+            attention_packed(q, k, k, cu, scale=scale)
+    for out in (q, z(4, 4, 32), z(4, 64, 4).transpose(1, 2), z(3, 4, 64)):
+        with pytest.raises(ValueError):
+            attention_packed(q, k, k, cu, out=out)
+    grad = z(4, 4, 64).requires_grad_()
+    with pytest.raises(RuntimeError, match="no_grad"):
+        attention_packed(grad, k, k, cu)
+    with torch.no_grad():
+        attention_packed(grad, k, k, cu)
+    pos, (freq, _) = torch.zeros(4, dtype=torch.int32, device="cuda"), rotary_frequencies(64)
+    for args in ((q, z(5, 2, 64), pos, freq), (q, k, pos[:3], freq), (q, k, pos, torch.cat([freq, freq])), (q, k, pos.cpu(), freq), (q, k, pos, freq[:0])):
+        with pytest.raises(ValueError):
+            rotate_heads(*args)
+    for args in ((q, k, pos.float(), freq), (q, k, pos, freq.float())):
+        with pytest.raises(TypeError):
+            rotate_heads(*args)
+    whole = z(5, 4, 64)
+    with pytest.raises(ValueError, match="overlaps"):
+        rotate_heads(whole[:4], None, pos, freq, out=(whole[1:], None))
+    with pytest.raises(RuntimeError, match="no_grad"):
+        rotate_heads(grad, k, pos, freq)
+    x, v = z(4, 64), z(64)
+    rows = torch.zeros(4, dtype=torch.int32, device="cuda")
+    for kw in (dict(post_weight=v), dict(mod_scale=v), dict(gate=z(65)), dict(weight=z(63)), dict(eps=-1.0), dict(vector_rows=rows), dict(gate=v, vector_rows=rows),
+               dict(gate=z(2, 64), mod_scale=z(3, 64), mod_shift=z(3, 64), vector_rows=rows), dict(gate=z(2, 64), vector_rows=rows[:3])):
+        with pytest.raises(ValueError):
+            residual_norm_quantize_rows(x, x, **kw)
+    for kw in (dict(weight=v.float()), dict(gate=v.cpu()), dict(gate=z(2, 64), vector_rows=rows.long())):
+        with pytest.raises(TypeError):
+            residual_norm_quantize_rows(x, x, **kw)
+    with pytest.raises(ValueError):
+        residual_norm_quantize_rows(x, z(3, 64))
+    empty = residual_norm_quantize_rows(z(0, 64), z(0, 64))
+    assert [t.shape for t in empty] == [(0, 64), (0, 64), (0, 1)]
+
+
+def test_no_wait_has_run_out():
+    import ctypes
+    from sacq_b200 import _lib
+    word = ctypes.c_int(-1)
+    _lib.check(_lib.load().sacq_block_steps_status(ctypes.byref(word)))
+    assert word.value == 0
