@@ -177,6 +177,7 @@ bool attention_tma_supported(const AttnParams& p);
 AttnSplit attention_split(const AttnParams& a, int64_t items, int64_t items_per_sequence, int64_t slots, int min_chunk, void* workspace);
 int64_t attention_split_bytes(const AttnParams& a, const AttnSplit& split);
 int attention_tensor_maps(const AttnParams& a, int q_box_heads, int q_box_tokens, int k_box_tokens, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v);
+int attention_out_map(const AttnParams& a, int box_heads, int box_tokens, CUtensorMap* out);
 int device_sms();
 
 // Tensor cores by tcgen05: tiles of 128 query rows.

@@ -98,7 +98,7 @@ int attention_status(int* out) {
 bool attention_tma_supported(const AttnParams& a) {
   auto al = [](const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
   return a.dim <= 128 && a.dim % 8 == 0 && a.tokens_k > 0 && al(a.q, 16) && al(a.k, 16) && al(a.v, 16) && al(a.out, 16) &&
-         a.out_token % 8 == 0 && a.out_head % 8 == 0 && strides_for_tma(a.q_token, a.q_head, a.heads, a.tokens_q) &&
+         strides_for_tma(a.out_token, a.out_head, a.heads, a.tokens_q) && strides_for_tma(a.q_token, a.q_head, a.heads, a.tokens_q) &&
          strides_for_tma(a.k_token, a.k_head, a.kv_heads, a.tokens_k) && strides_for_tma(a.v_token, a.v_head, a.kv_heads, a.tokens_k);
 }
 
@@ -130,17 +130,24 @@ int64_t attention_split_bytes(const AttnParams& a, const AttnSplit& s) {
   return s.chunks_most == 1 ? 0 : lse_offset(a, s.chunks_most) + (int64_t)s.chunks_most * a.tokens_q * a.heads * 4;
 }
 
+namespace {
+int heads_map(CUtensorMap* m, const AttnParams& a, const void* base, int64_t tokens, int heads, int64_t token, int64_t head, int box_heads, int box_tokens) {
+  // the stride of a dimension of one element means nothing, but is checked
+  const int64_t h = heads == 1 ? a.dim : head, t = tokens == 1 ? (int64_t)a.dim * heads : token;
+  return encode_bf16_3d(m, base, (uint64_t)a.dim, (uint64_t)heads, (uint64_t)tokens, (uint64_t)h, (uint64_t)t, 64u, (uint32_t)box_heads,
+                        (uint32_t)box_tokens, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+}  // namespace
+
 int attention_tensor_maps(const AttnParams& a, int q_box_heads, int q_box_tokens, int k_box_tokens, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v) {
-  auto make = [&](CUtensorMap* m, const void* base, int64_t tokens, int heads, int64_t token, int64_t head, int box_heads, int box_tokens) {
-    // the stride of a dimension of one element means nothing, but is checked
-    const int64_t h = heads == 1 ? a.dim : head, t = tokens == 1 ? (int64_t)a.dim * heads : token;
-    return encode_bf16_3d(m, base, (uint64_t)a.dim, (uint64_t)heads, (uint64_t)tokens, (uint64_t)h, (uint64_t)t, 64u, (uint32_t)box_heads,
-                          (uint32_t)box_tokens, CU_TENSOR_MAP_SWIZZLE_128B);
-  };
   if (q != nullptr)
-    if (int rc = make(q, a.q, a.tokens_q, a.heads, a.q_token, a.q_head, q_box_heads, q_box_tokens)) return rc;
-  if (int rc = make(k, a.k, a.tokens_k, a.kv_heads, a.k_token, a.k_head, 1, k_box_tokens)) return rc;
-  return make(v, a.v, a.tokens_k, a.kv_heads, a.v_token, a.v_head, 1, k_box_tokens);
+    if (int rc = heads_map(q, a, a.q, a.tokens_q, a.heads, a.q_token, a.q_head, q_box_heads, q_box_tokens)) return rc;
+  if (int rc = heads_map(k, a, a.k, a.tokens_k, a.kv_heads, a.k_token, a.k_head, 1, k_box_tokens)) return rc;
+  return heads_map(v, a, a.v, a.tokens_k, a.kv_heads, a.v_token, a.v_head, 1, k_box_tokens);
+}
+
+int attention_out_map(const AttnParams& a, int box_heads, int box_tokens, CUtensorMap* out) {
+  return heads_map(out, a, a.out, a.tokens_q, a.heads, a.out_token, a.out_head, box_heads, box_tokens);
 }
 
 int launch_attention_join(const AttnParams& a, const AttnSplit& split, cudaStream_t s) {

@@ -75,6 +75,9 @@ struct Shape {
 constexpr int Q_FULL = 0, Q_EMPTY = 1, S_FULL = 2, P_FULL = 4, O_FULL = 6, ITEM_FULL = 10, ITEM_EMPTY = 12,
               DRAIN = 14, TAKE = 15, KV_FULL = 16, KV_EMPTY = 32, JOIN_FULL = 48, JOIN_EMPTY = 52;
 
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int x, int y, int z, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(src) : "memory");
+}
 __device__ __forceinline__ void umma_bf16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -225,7 +228,8 @@ __device__ __forceinline__ int columns(int most, int j) { return (min(kTile, mos
 template <int DP>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TmemAttnParams p) {
+                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o,
+                      const __grid_constant__ TmemAttnParams p) {
   using Sh = Shape<DP>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t sm = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -272,6 +276,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     prefetch_tensormap(&map_q);
     prefetch_tensormap(&map_k);
     prefetch_tensormap(&map_v);
+    prefetch_tensormap(&map_o);
   }
   tc_fence_before();
   __syncthreads();
@@ -527,6 +532,8 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       it.dual = (int)warp_uniform(it.dual); it.part = (int)warp_uniform(it.part);
       if (lane == 0) mbar_arrive(bar(ITEM_EMPTY + (i & 1)));
       if (it.last) break;
+      // this warp's copies out have read their room: where a lone tile's sums will be handed over
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       const int t = (row >> p.pack_log2) + (it.dual ? w * tile_tokens : 0);      // token of the item
       const bool valid = t < it.q_left;
       const bool live = __any_sync(0xffffffffu, valid);
@@ -656,6 +663,9 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       // rows leave through shared memory, 128 bytes of each at a time, so that a store covers 4 rows' lines and not 32
       uint8_t* const stage = sp + Sh::kJoin + quarter * 8192 + w * 4096;
       if (w == 1 && !mbar_wait_warp(bar(JOIN_EMPTY + quarter), (nj & 1) ^ 1, abort_flag, p.status)) break;      // its own sums have been read
+      // first token of the warp's rows; rows of 32 real queries go by one copy, others one by one
+      const int slice = (quarter * 32 >> p.pack_log2) + (it.dual ? w * tile_tokens : 0);
+      const bool whole = p.pack_log2 <= 5 && slice + (32 >> p.pack_log2) <= it.q_left;
       float inv = 0.f, scale0 = 1.f, scale1 = 0.f;
       bool finite = true;
 #pragma unroll 1
@@ -716,20 +726,31 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           for (int e = 0; e < 64; ++e) o[e >> 5][e & 31] = 0u;
         }
         if (it.part < 0) {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");    // the last copy from here has read it
+          __syncwarp();
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const float* const f = reinterpret_cast<const float*>(&o[e >> 2][8 * (e & 3)]);
             *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ (lane & 7)) << 4)) =
                 make_uint4(bf16_pair(f[0], f[1]), bf16_pair(f[2], f[3]), bf16_pair(f[4], f[5]), bf16_pair(f[6], f[7]));
           }
-          __syncwarp();
+          if (whole) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(&map_o, h * 64, it.head, it.q_row + slice, sm + (uint32_t)(stage - sp));
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+          } else {
+            __syncwarp();
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int r = e * 4 + (lane >> 3), piece = lane & 7, rr = quarter * 32 + r;
-            const int tt = (rr >> p.pack_log2) + (it.dual ? w * tile_tokens : 0), d = h * 64 + piece * 8;
-            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((piece ^ (r & 7)) << 4));
-            if (tt < it.q_left && d < a.dim)
-              *reinterpret_cast<uint4*>(a.out + ((int64_t)it.q_row + tt) * a.out_token + (int64_t)(it.head + (rr & ((1 << p.pack_log2) - 1))) * a.out_head + d) = v;
+            for (int e = 0; e < 8; ++e) {
+              const int r = e * 4 + (lane >> 3), piece = lane & 7, rr = quarter * 32 + r;
+              const int tt = (rr >> p.pack_log2) + (it.dual ? w * tile_tokens : 0), d = h * 64 + piece * 8;
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((piece ^ (r & 7)) << 4));
+              if (tt < it.q_left && d < a.dim)
+                *reinterpret_cast<uint4*>(a.out + ((int64_t)it.q_row + tt) * a.out_token + (int64_t)(it.head + (rr & ((1 << p.pack_log2) - 1))) * a.out_head + d) = v;
+            }
           }
         } else if (valid) {
           float* const po = p.split.part_o + slot * a.dim + h * 64;
@@ -740,7 +761,10 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           }
         }
         __syncwarp();
-        if (joined && lane == 0) mbar_arrive(bar(JOIN_EMPTY + quarter));
+        if (joined && lane == 0) {           // the copy has read what the next half will overwrite
+          asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          mbar_arrive(bar(JOIN_EMPTY + quarter));
+        }
       }
       if (!ok) break;
       if (valid) {
@@ -753,6 +777,8 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       __syncwarp();                          // the rows as they are lie in front of the ones made again
       uint32_t odd = __ballot_sync(0xffffffffu, valid && !finite);
       if (odd != 0) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
         const int most = seen(it, causal, min(it.q_left, (it.dual && w == 1 ? 2 : 1) * tile_tokens) - 1);
         odd = __ballot_sync(0xffffffffu, valid && !finite && mine < min((most + 15) & ~15, it.keys));
       }
@@ -764,6 +790,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       }
     }
   }
+  if (warp < kMmaWarp && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   // ---- common exit: every thread arrives here, also after an aborted wait
   tc_fence_before();
   __syncthreads();
@@ -804,9 +831,10 @@ int launch_attention_tmem(const AttnParams& a, const AttnSplit& split, cudaStrea
   p.status = attention_status_word();
   if (p.status == nullptr) return set_error(SACQ_ERR_CUDA, "no status word on this device");
   const int64_t most = t.items * split.chunks_most;
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mk, mv, mo;
   const int pack = 1 << t.pack_log2;
   if (int rc = attention_tensor_maps(a, pack, kTile / pack, kTile, &mq, &mk, &mv)) return rc;
+  if (int rc = attention_out_map(a, pack < 32 ? pack : 32, pack < 32 ? 32 / pack : 1, &mo)) return rc;
   const bool wide = a.dim > 64;
   const void* fn = wide ? (const void*)attention_tmem_kernel<128> : (const void*)attention_tmem_kernel<64>;
   const size_t smem = (wide ? Shape<128>::kTotal : Shape<64>::kTotal) + 1024;
@@ -830,7 +858,7 @@ int launch_attention_tmem(const AttnParams& a, const AttnSplit& split, cudaStrea
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  void* args[] = {&mq, &mk, &mv, &p};
+  void* args[] = {&mq, &mk, &mv, &mo, &p};
   SACQ_CUDA_TRY(cudaLaunchKernelExC(&cfg, fn, args));
   count_launch();
   return SACQ_OK;
