@@ -35,18 +35,26 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
   float l = 0.f;
   float o[4] = {0.f, 0.f, 0.f, 0.f};
   const int d = lane * 4;
-#pragma unroll 4
-  for (int i = 0; i < chunks; ++i) {
-    const float le = split.part_lse[i * stride + at];
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (d < a.dim) v = *reinterpret_cast<const float4*>(split.part_o + (i * stride + at) * a.dim + d);
-    if (le == -INFINITY) continue;           // the query sees none of its keys
-    const float f = exp2f((le - base) * kLog2e);
-    l += f;
-    o[0] = fmaf(v.x, f, o[0]);
-    o[1] = fmaf(v.y, f, o[1]);
-    o[2] = fmaf(v.z, f, o[2]);
-    o[3] = fmaf(v.w, f, o[3]);
+  const float* const src = split.part_o + at * a.dim + (d < a.dim ? d : 0);
+  for (int first = 0; first < chunks; first += 32) {
+    // this lane's chunk's weight: 0 where the query sees none of its keys, whose part is zeros
+    const int n = min(32, chunks - first);
+    const float f = lane < n ? exp2f((split.part_lse[(first + lane) * stride + at] - base) * kLog2e) : 0.f;
+    for (int i = 0; i < n; i += 8) {         // eight parts are on their way at a time
+      float4 v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const float4*>(src + (first + min(i + e, n - 1)) * stride * a.dim);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float w = __shfl_sync(0xffffffffu, f, min(i + e, 31));
+        if (i + e >= n) break;
+        l += w;
+        o[0] = fmaf(v[e].x, w, o[0]);
+        o[1] = fmaf(v[e].y, w, o[1]);
+        o[2] = fmaf(v[e].z, w, o[2]);
+        o[3] = fmaf(v[e].w, w, o[3]);
+      }
+    }
   }
   const bool some = l != 0.f;                // a NaN is some, too
   if (d < a.dim) {

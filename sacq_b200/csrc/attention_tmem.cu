@@ -566,10 +566,13 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             }
             if (masked) {                    // columns that this row does not see
 #pragma unroll
-              for (int b = 2 * h; b < 2 * h + 2; ++b)
+              for (int b = 2 * h; b < 2 * h + 2; ++b) {
+                const int left = end - b * 32;
+                const uint32_t visible = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
 #pragma unroll
                 for (int e = 0; e < 32; ++e)
-                  if (b * 32 + e >= end) s[b][e] = 0xff800000u;
+                  if ((visible & (1u << e)) == 0) s[b][e] = 0xff800000u;
+              }
             }
 #pragma unroll
             for (int b = 2 * h; b < 2 * h + 2; ++b)
