@@ -170,8 +170,8 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
 }
 // 2^x of two values: on the special-function unit, or by a polynomial.  The unit takes 8 cycles for a warp, which would
 // bound the kernel; of every 8 pairs kPolynomials go by x = n + f, f in [-1/2, 1/2], and a polynomial of degree 5 for 2^f (least
-// largest relative error, 7.5e-8, fitted by iterated reweighted least squares), n added to its exponent.  Below 2^-126 the
-// result is that power: such weights count for nothing beside the row's largest.
+// largest relative error, 7.5e-8, fitted by iterated reweighted least squares), n added to its exponent.  From x = -127 down, -inf
+// among them, that leaves 2^-149, which is zero in bf16: a weight of a column that is not seen has to be, whatever V holds there.
 constexpr int kPolynomials = 2;
 __device__ __forceinline__ uint64_t exp2_unit(uint64_t v) {
   float x, y;
@@ -181,7 +181,7 @@ __device__ __forceinline__ uint64_t exp2_unit(uint64_t v) {
 __device__ __forceinline__ uint64_t exp2_polynomial(uint64_t v) {
   float x, y;
   halves_of(v, x, y);
-  v = f32x2(fmaxf(x, -126.f), fmaxf(y, -126.f));
+  v = f32x2(fmaxf(x, -127.f), fmaxf(y, -127.f));
   const uint64_t magic = f32x2(12582912.0f, 12582912.0f);            // 1.5 * 2^23: the sum holds the nearest integer in its low bits
   const uint64_t t = add2(v, magic);
   const uint64_t f = fma2(add2(t, f32x2(-12582912.0f, -12582912.0f)), f32x2(-1.f, -1.f), v);

@@ -168,7 +168,7 @@ def test_attention_reads_views_where_they_lie(dim):
 
 
 @pytest.mark.parametrize("heads,dim", (((4, 2), 128), ((2, 2), 64), ((2, 1), 36)))
-@pytest.mark.parametrize("value", (NAN, INF, -INF))
+@pytest.mark.parametrize("value", (NAN, INF, -INF, 3e38))
 def test_attention_keeps_what_is_not_seen_out(value, heads, dim):
     """Rows of no sequence, of other sequences and of later tokens may hold anything."""
     from sacq_b200 import attention_packed
