@@ -66,6 +66,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         _heads(out, "out")
         if out.shape != q.shape or out.device != q.device or (out.stride(2) != 1 and d > 1):
             raise ValueError("out must have q's shape and device, and a unit inner stride")
+        if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+            raise ValueError("out has elements that share memory")
         if _lib.native().overlaps(out, (q, k, v)):
             raise ValueError("out may not overlap q, k or v")
     q, k, v = (t if t.stride(2) == 1 or d == 1 else t.contiguous() for t in (q, k, v))

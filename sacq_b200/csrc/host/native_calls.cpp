@@ -16,6 +16,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
@@ -507,15 +508,37 @@ const at::Tensor* heads_of(PyObject* o, int dev) {
   return t;
 }
 
-// Bytes between the first and the last element
+// Whether two tensors share memory.  Views of one buffer whose elements take turns (the query and the key heads of a fused
+// projection) do not: where a stride S of either divides the larger strides of both, their places modulo S are two spans, and those
+// may lie apart.
 bool overlap(const at::Tensor& a, const at::Tensor& b) {
-  auto end = [](const at::Tensor& t) {
-    int64_t last = 0;
-    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
-    return (const char*)t.data_ptr() + (last + 1) * t.element_size();
-  };
   if (a.numel() == 0 || b.numel() == 0) return false;
-  return (const char*)a.data_ptr() < end(b) && (const char*)b.data_ptr() < end(a);
+  const at::Tensor* const both[2] = {&a, &b};
+  auto places = [&](int64_t step, int64_t (&span)[2]) {      // bytes from a tensor's first to its last place modulo `step` bytes
+    for (int t = 0; t < 2; ++t) {
+      const int64_t size = both[t]->element_size();
+      span[t] = size;
+      for (int64_t i = 0; i < both[t]->dim(); ++i) {
+        const int64_t stride = both[t]->stride(i) * size;
+        if (both[t]->size(i) == 1 || (step != 0 && stride % step == 0)) continue;
+        if (step != 0 && stride > step) return false;
+        span[t] += (both[t]->size(i) - 1) * stride;
+      }
+    }
+    return true;
+  };
+  const char *const pa = (const char*)a.data_ptr(), *const pb = (const char*)b.data_ptr();
+  int64_t span[2];
+  places(0, span);
+  if (pa >= pb + span[1] || pb >= pa + span[0]) return false;
+  for (const at::Tensor* t : both)
+    for (int64_t i = 0; i < t->dim(); ++i) {
+      const int64_t step = t->stride(i) * t->element_size();
+      if (t->size(i) == 1 || step <= 0 || !places(step, span)) continue;
+      const int64_t apart = ((pb - pa) % step + step) % step;
+      if (apart >= span[0] && apart + span[1] <= step) return false;
+    }
+  return true;
 }
 
 // overlaps(a, (b, ...))
@@ -544,6 +567,9 @@ PyObject* tuple_of(std::initializer_list<at::Tensor> list) {
   }
   return t;
 }
+
+// A result that can be written: no two of its elements are one
+bool writable(const at::Tensor& t) { return at::has_internal_overlap(t) != at::MemOverlap::Yes; }
 
 bool offsets_of(const at::Tensor* t, int dev) {
   return t != nullptr && t->scalar_type() == at::kInt && on_device(*t, dev) && t->dim() == 1 && t->numel() >= 1 && t->is_contiguous();
@@ -574,7 +600,7 @@ PyObject* py_attention_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
     out = new_tensor({q->size(0), h, d}, at::kBFloat16, dev);
   } else {
     const at::Tensor* o = heads_of(a[7], dev);
-    if (o == nullptr || o->sizes() != q->sizes() || overlap(*o, *q) || overlap(*o, *k) || overlap(*o, *v)) Py_RETURN_NONE;
+    if (o == nullptr || o->sizes() != q->sizes() || !writable(*o) || overlap(*o, *q) || overlap(*o, *k) || overlap(*o, *v)) Py_RETURN_NONE;
     out = *o;
   }
   const bool want_lse = a[8] == Py_True;
@@ -614,14 +640,15 @@ PyObject* py_attention_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NATIVE_CATCH
 }
 
-bool fill_heads(const at::Tensor* x, PyObject* out_obj, int dev, sacq_head_rows& r, at::Tensor& out) {
+// other: the call's other input, null if there is none.  In place means the same places, so `other` is still looked at
+bool fill_heads(const at::Tensor* x, const at::Tensor* other, PyObject* out_obj, int dev, sacq_head_rows& r, at::Tensor& out) {
   if (out_obj == Py_None) {
     out = new_tensor(x->sizes(), at::kBFloat16, dev);
   } else {
     const at::Tensor* o = heads_of(out_obj, dev);
-    if (o == nullptr || o->sizes() != x->sizes()) return false;
+    if (o == nullptr || o->sizes() != x->sizes() || !writable(*o)) return false;
     const bool same = o->data_ptr() == x->data_ptr() && o->strides() == x->strides();
-    if (!same && overlap(*o, *x)) return false;
+    if ((!same && overlap(*o, *x)) || (other != nullptr && overlap(*o, *other))) return false;
     out = *o;
   }
   r.in = x->data_ptr();
@@ -654,7 +681,8 @@ PyObject* py_rotate_heads(PyObject*, PyObject* const* a, Py_ssize_t n) {
   sacq_rotary_desc c = {};
   c.struct_size = sizeof(c);
   at::Tensor q_out, k_out;
-  if (!fill_heads(q, a[6], dev, c.q, q_out) || (k != nullptr && !fill_heads(k, a[7], dev, c.k, k_out))) Py_RETURN_NONE;
+  if (!fill_heads(q, k, a[6], dev, c.q, q_out) || (k != nullptr && !fill_heads(k, q, a[7], dev, c.k, k_out))) Py_RETURN_NONE;
+  if (k != nullptr && a[6] != Py_None && a[7] != Py_None && overlap(q_out, k_out)) Py_RETURN_NONE;
   c.layout = (int32_t)PyLong_AsLong(a[4]);
   c.tokens = q->size(0);
   c.head_dim = (int32_t)q->size(2);

@@ -74,7 +74,7 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     ``q``, ``k`` (or ``None``): bf16 ``[tokens, heads, head_dim]``, any strides with a unit inner one.  ``positions``: int32 or int64
     ``[tokens]``; ``inv_freq``: float64 ``[rotary_dim / 2]`` (``rotary_frequencies``); ``rotary_dim`` is at most ``head_dim`` and what lies behind it
     is copied.  ``layout``: ``"half"`` pairs element ``i`` with ``i + rotary_dim / 2``, ``"interleaved"`` ``2 i`` with ``2 i + 1``.
-    ``out=(q_out, k_out)`` receives the results; ``out=(q, k)`` turns in place.  Angles are made in double: positions of any size are as exact as
+    ``out=(q_out, k_out)`` receives the results; ``out=(q, k)`` turns in place, views of one fused buffer too.  Angles are made in double: positions of any size are as exact as
     small ones."""
     if layout not in _LAYOUTS:
         raise ValueError(f"unknown layout {layout!r}")
@@ -101,15 +101,19 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         raise ValueError(f"{inv_freq.numel()} pairs do not fit heads of {d}")
     if k is None and k_out is not None:
         raise ValueError("there is no k for out[1]")
-    for x, y, what in ((q, q_out, "out[0]"), (k, k_out, "out[1]")):
+    for x, other, y, what in ((q, k, q_out, "out[0]"), (k, q, k_out, "out[1]")):
         if y is None:
             continue
         _heads(y, what)
         if y.shape != x.shape or y.device != x.device or (y.stride(2) != 1 and d > 1):
             raise ValueError(f"{what} must have the shape and device of its input, and a unit inner stride")
         same = y.data_ptr() == x.data_ptr() and y.stride() == x.stride()
-        if not same and _lib.native().overlaps(y, (x,)):
-            raise ValueError(f"{what} overlaps its input without being it")
+        if any(n > 1 and s == 0 for n, s in zip(y.shape, y.stride())):
+            raise ValueError(f"{what} has elements that share memory")
+        if _lib.native().overlaps(y, (other,) if same else (x, other)):
+            raise ValueError(f"{what} overlaps an input that it does not replace")
+    if q_out is not None and k_out is not None and _lib.native().overlaps(q_out, (k_out,)):
+        raise ValueError("the results overlap each other")
     q, k = (x if x is None or x.stride(2) == 1 or d == 1 else x.contiguous() for x in (q, k))
     made = _lib.native().rotate_heads(q, k, positions.contiguous(), inv_freq.contiguous(), _LAYOUTS[layout], float(amplitude),
                                       q_out, k_out)

@@ -120,3 +120,24 @@ def test_rotary_frequencies():
                     (8, {"scaling": {"kind": "wavelength", "factor": 2.0, "original": 4096, "low": 4.0, "high": 4.0}})):
         with pytest.raises(ValueError):
             rotary_frequencies(dim, device="cpu", **kw)
+
+
+def test_views_overlap_where_they_share_elements():
+    overlaps = _lib.native().overlaps
+    x = torch.zeros(6, 12, 8)
+    apart = ((x[:, :4], x[:, 4:8]), (x[:3], x[3:]), (x[:, ::2], x[:, 1::2]), (x[:, :, :4], x[:, :, 4:]), (x[::2], x[1::2]), (x[:, 3:5], x[:, 5:]),
+             (x[:, 8:, :2], x[:, :8, 1:]), (x[:0], x), (x[:, :1], x[:, 1:]), (x[:1, ::2], x[:1, 1::2]))
+    shared = ((x, x), (x[:, :5], x[:, 4:8]), (x[:4], x[3:]), (x[:, ::2], x[:, ::3]), (x[:, :, :5], x[:, :, 4:]), (x[1], x[:, 3:4]), (x[:, 1:2], x[:, :4]))
+    for pairs, want in ((apart, False), (shared, True)):
+        for a, b in pairs:
+            assert overlaps(a, (b,)) is want and overlaps(b, (a,)) is want and overlaps(a, (None, b)) is want
+    # against the elements themselves, over small views; what shares must be found, what does not may be called shared
+    storage, found = torch.arange(400), 0
+    rng = torch.Generator().manual_seed(5)
+    for _ in range(2000):
+        n = lambda hi: int(torch.randint(1, hi, (1,), generator=rng))
+        views = [storage.as_strided((n(4), n(4), n(4)), (n(30), n(12), 1), n(60)) for _ in range(2)]
+        share = bool(set(views[0].flatten().tolist()) & set(views[1].flatten().tolist()))
+        found += share
+        assert overlaps(views[0], (views[1],)) or not share
+    assert 100 < found < 1900

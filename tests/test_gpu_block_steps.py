@@ -582,6 +582,25 @@ def test_policy_of_prompts_of_different_lengths():
             policy.forward_packed(image, noise, bad)
 
 
+def test_rotary_results_lie_in_one_buffer_of_any_order():
+    from sacq_b200 import rotary_frequencies, rotate_heads
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    t, h, d = 37, 3, 64
+    q, k = _randn(gen, t, h, d), _randn(gen, t, h, d)
+    pos, (freq, _) = torch.arange(t, device="cuda"), rotary_frequencies(d)
+    want = rotate_heads(q, k, pos, freq)
+    for views in (lambda x: (x[:, :h], x[:, h:]), lambda x: (x[:, ::2], x[:, 1::2])):
+        made = torch.zeros(t, 2 * h, d, device="cuda", dtype=torch.bfloat16)
+        rotate_heads(q, k, pos, freq, out=views(made))
+        turned = torch.zeros_like(made)
+        views(turned)[0].copy_(q)
+        views(turned)[1].copy_(k)
+        rotate_heads(*views(turned), pos, freq, out=views(turned))
+        for x in (made, turned):
+            assert all(torch.equal(a, b) for a, b in zip(views(x), want))
+    assert all(torch.equal(a, b) for a, b in zip(rotate_heads(q, q, pos, freq), (want[0], want[0])))
+
+
 def test_steps_refuse_what_they_cannot_do():
     from sacq_b200 import attention_packed, residual_norm_quantize_rows, rotary_frequencies, rotate_heads
     z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
@@ -596,7 +615,7 @@ def test_steps_refuse_what_they_cannot_do():
     for scale in (0.0, -1.0, INF, NAN):
         with pytest.raises(ValueError):
             attention_packed(q, k, k, cu, scale=scale)
-    for out in (q, z(4, 4, 32), z(4, 64, 4).transpose(1, 2), z(3, 4, 64)):
+    for out in (q, z(4, 4, 32), z(4, 64, 4).transpose(1, 2), z(3, 4, 64), z(1, 4, 64).expand(4, 4, 64)):
         with pytest.raises(ValueError):
             attention_packed(q, k, k, cu, out=out)
     grad = z(4, 4, 64).requires_grad_()
@@ -614,6 +633,13 @@ def test_steps_refuse_what_they_cannot_do():
     whole = z(5, 4, 64)
     with pytest.raises(ValueError, match="overlaps"):
         rotate_heads(whole[:4], None, pos, freq, out=(whole[1:], None))
+    two = z(4, 4, 64)
+    for out in ((two, q), (two, two), (two, None), (None, q), (z(1, 4, 64).expand(4, 4, 64), None)):
+        with pytest.raises(ValueError):
+            rotate_heads(q, two, pos, freq, out=out)
+    for out in ((q, None), (None, q), (q, q)):                    # the same heads twice, one of them turned in place
+        with pytest.raises(ValueError, match="overlap"):
+            rotate_heads(q, q, pos, freq, out=out)
     with pytest.raises(RuntimeError, match="no_grad"):
         rotate_heads(grad, k, pos, freq)
     x, v = z(4, 64), z(64)
