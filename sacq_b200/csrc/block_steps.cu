@@ -123,7 +123,8 @@ enum { kByRows, kShort, kTmem };
 // average is known here.
 int attention_kernel(const AttnParams& p) {
   if (!attention_tma_supported(p)) return kByRows;
-  return p.tokens_q * (p.heads / p.kv_heads) <= 32 * (int64_t)p.sequences ? kShort : kTmem;
+  const int64_t rows = p.tokens_q * (p.heads / p.kv_heads);
+  return rows <= 32 * (int64_t)p.sequences && rows < (1ll << 31) - 64 ? kShort : kTmem;
 }
 AttnSplit split_for(const AttnParams& p, int kernel, void* workspace) {
   return kernel == kShort ? attention_short_split(p, workspace) : attention_tmem_split(p, workspace);

@@ -657,6 +657,34 @@ def test_steps_refuse_what_they_cannot_do():
     assert [t.shape for t in empty] == [(0, 64), (0, 64), (0, 1)]
 
 
+def test_the_first_call_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+    code = """
+import torch
+from sacq_b200 import attention_packed, residual_norm_quantize_rows, rotary_frequencies, rotate_heads
+g = torch.Generator(device="cuda").manual_seed(0)
+r = lambda *s: torch.randn(*s, generator=g, device="cuda").to(torch.bfloat16)
+q, k, v, x, y = r(3000, 4, 64), r(3000, 2, 64), r(3000, 2, 64), r(3000, 256), r(3000, 256)
+cu = torch.tensor([0, 1000, 3000], dtype=torch.int32, device="cuda")
+one = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+pos, (freq, _) = torch.arange(3000, device="cuda"), rotary_frequencies(64)
+def calls():
+    a, b = rotate_heads(q, k, pos, freq)
+    return [a, b, attention_packed(a, b, v, cu, causal=True), attention_packed(q[:2], k, v, one, cu), *residual_norm_quantize_rows(x, y)[::2]]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    made = calls()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(m, e) for m, e in zip(made, calls()))
+print("same")
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
+
+
 def test_no_wait_has_run_out():
     import ctypes
     from sacq_b200 import _lib
