@@ -49,19 +49,38 @@ __device__ void attend_row(const AttnParams& p, const uint16_t* q, const uint16_
   }
   st.m = -INFINITY;
   st.l = 0.f;
-  for (int64_t j = 0; j < keys; ++j) {
-    float s = 0.f;
+  constexpr int kAtOnce = 4;                 // scores whose sums over the lanes run together
+  for (int64_t j = 0; j < keys; j += kAtOnce) {
+    float s[kAtOnce];
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (lane + 32 * e < p.dim) s = fmaf(qe[e], bf16_bits_to_float(k[j * p.k_token + lane + 32 * e]), s);
-    s = warp_sum(s);
-    const float m = fmaxf(st.m, s), base = m == -INFINITY ? 0.f : m;
-    const float keep = expf(st.m - base), w = expf(s - base);
+    for (int i = 0; i < kAtOnce; ++i) {
+      s[i] = 0.f;
+      const uint16_t* const row = k + min(j + i, keys - 1) * p.k_token;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (lane + 32 * e < p.dim) s[i] = fmaf(qe[e], bf16_bits_to_float(row[lane + 32 * e]), s[i]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
+    float m = st.m;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) m = fmaxf(m, s[i]);
+    const float base = m == -INFINITY ? 0.f : m, keep = expf(st.m - base);
     st.m = m;
-    st.l = st.l * keep + w;
+    st.l *= keep;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (lane + 32 * e < p.dim) st.acc[e] = fmaf(st.acc[e], keep, w * bf16_bits_to_float(v[j * p.v_token + lane + 32 * e]));
+    for (int e = 0; e < E; ++e) st.acc[e] *= keep;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (j + i >= keys) break;
+      const float w = expf(s[i] - base);
+      st.l += w;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (lane + 32 * e < p.dim) st.acc[e] = fmaf(w, bf16_bits_to_float(v[(j + i) * p.v_token + lane + 32 * e]), st.acc[e]);
+    }
   }
 }
 
@@ -79,6 +98,8 @@ __device__ __forceinline__ int chunks_of(const AttnSplit& s, int keys) {
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
+// Waits of these kernels: a warp that makes 32 rows again (redo_row) is at it for 60 clocks a row and key, others wait meanwhile.
+constexpr uint64_t kWaitNs = 10000000000ull;
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

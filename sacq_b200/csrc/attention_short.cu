@@ -133,7 +133,7 @@ attention_short_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         const int most = causal ? min(it.keys, it.base + (min(it.first + kRows, it.q_rows) - 1) / group + 1) : it.keys;
         it.steps = most > 0 ? (most + kStep - 1) / kStep : 0;
       }
-      ok = mbar_wait_warp(bar(IT_EMPTY + (made & 1)), ((made >> 1) & 1) ^ 1, abort_flag, p.status);
+      ok = mbar_wait_warp(bar(IT_EMPTY + (made & 1)), ((made >> 1) & 1) ^ 1, abort_flag, p.status, kWaitNs);
       if (!ok) break;
       const int rows = it.last ? 0 : min(kRows, it.q_rows - it.first);
       if (lane == 0) {
@@ -151,7 +151,7 @@ attention_short_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       if (it.last) break;
       for (int j = 0; j < it.steps; ++j, ++c) {
         const uint32_t s = c % Sh::kStages;
-        ok = mbar_wait_warp(bar(ST_EMPTY + s), ((c / Sh::kStages) & 1) ^ 1, abort_flag, p.status);
+        ok = mbar_wait_warp(bar(ST_EMPTY + s), ((c / Sh::kStages) & 1) ^ 1, abort_flag, p.status, kWaitNs);
         if (!ok) break;
         if (elect_one()) {
           mbar_arrive_expect_tx(bar(ST_FULL + s), Sh::kStageBytes);
@@ -186,11 +186,11 @@ attention_short_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
   auto meet = [&] {                          // of the four warps
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(JOIN));
-    ok = mbar_wait_warp(bar(JOIN), joins & 1, abort_flag, p.status) && ok;
+    ok = mbar_wait_warp(bar(JOIN), joins & 1, abort_flag, p.status, kWaitNs) && ok;
     ++joins;
   };
   for (uint32_t i = 0; ok; ++i) {
-    if (!mbar_wait_warp(bar(IT_FULL + (i & 1)), (i >> 1) & 1, abort_flag, p.status)) break;
+    if (!mbar_wait_warp(bar(IT_FULL + (i & 1)), (i >> 1) & 1, abort_flag, p.status, kWaitNs)) break;
     const ShortItem it = *item_at(i);
     uint32_t q[DP / 16][4];
 #pragma unroll
@@ -216,7 +216,7 @@ attention_short_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     for (int j = 0; j < it.steps; ++j, ++c) {
       const uint32_t s = c % Sh::kStages;
-      if (!mbar_wait_warp(bar(ST_FULL + s), (c / Sh::kStages) & 1, abort_flag, p.status)) { ok = false; break; }
+      if (!mbar_wait_warp(bar(ST_FULL + s), (c / Sh::kStages) & 1, abort_flag, p.status, kWaitNs)) { ok = false; break; }
       const int key = j * kStep + keys_from;                 // first of this warp's
       if (key < most) {
         const uint32_t kt = sm + s * Sh::kStageBytes, vt = kt + Sh::kTensorBytes;

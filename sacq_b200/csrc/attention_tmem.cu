@@ -290,7 +290,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     bool ok = true;
     auto take = [&](const CUtensorMap* map, const Item& it, int j) {
       const uint32_t s = c % Sh::kStages;
-      ok = ok && mbar_wait_warp(bar(KV_EMPTY + s), ((c / Sh::kStages) & 1) ^ 1, abort_flag, p.status);
+      ok = ok && mbar_wait_warp(bar(KV_EMPTY + s), ((c / Sh::kStages) & 1) ^ 1, abort_flag, p.status, kWaitNs);
       if (!ok) return;
       if (elect_one()) {
         mbar_arrive_expect_tx(bar(KV_FULL + s), Sh::kTileBytes);
@@ -322,7 +322,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         index += gridDim.x;
         return;
       }
-      ok = mbar_wait_warp(bar(TAKE), taken & 1, abort_flag, p.status);
+      ok = mbar_wait_warp(bar(TAKE), taken & 1, abort_flag, p.status, kWaitNs);
       ++taken;
       uint32_t cta = 0;
       more = ok && answered_cta(answer, cta);
@@ -358,7 +358,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         it.n0 = it.dual ? key_tiles(seen(it, causal, tile_tokens - 1)) : 0;
         it.part = chunks > 1 ? part : -1;
       }
-      ok = mbar_wait_warp(bar(ITEM_EMPTY + (made & 1)), ((made >> 1) & 1) ^ 1, abort_flag, p.status);
+      ok = mbar_wait_warp(bar(ITEM_EMPTY + (made & 1)), ((made >> 1) & 1) ^ 1, abort_flag, p.status, kWaitNs);
       if (!ok) break;
       if (lane == 0) *item_at(made) = it;
       __syncwarp();
@@ -367,7 +367,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       ++made;
       if (it.last) break;
       if (it.n == 0) continue;
-      ok = mbar_wait_warp(bar(Q_EMPTY), (nq & 1) ^ 1, abort_flag, p.status);
+      ok = mbar_wait_warp(bar(Q_EMPTY), (nq & 1) ^ 1, abort_flag, p.status, kWaitNs);
       if (!ok) break;
       ++nq;
       if (elect_one()) {
@@ -398,7 +398,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     bool ok = true;
     auto next = [&]() -> uint32_t {          // the next tile of the ring
       const uint32_t s = c % Sh::kStages;
-      ok = ok && mbar_wait_warp(bar(KV_FULL + s), (c / Sh::kStages) & 1, abort_flag, p.status);
+      ok = ok && mbar_wait_warp(bar(KV_FULL + s), (c / Sh::kStages) & 1, abort_flag, p.status, kWaitNs);
       ++c;
       return warp_uniform(s);
     };
@@ -423,7 +423,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       n = (int)warp_uniform(n); w = (int)warp_uniform(w); s = warp_uniform(s);
       const uint64_t vd = make_mn_desc(sm + Sh::kRing + s * Sh::kTileBytes, Sh::kHalfBytes);
       const uint32_t more = warp_uniform(first ? 0u : 1u);
-      ok = ok && mbar_wait_warp(bar(P_FULL + w), (w == 0 ? np0 : np1) & 1, abort_flag, p.status);
+      ok = ok && mbar_wait_warp(bar(P_FULL + w), (w == 0 ? np0 : np1) & 1, abort_flag, p.status, kWaitNs);
       if (!ok) return;
       tc_fence_after();
 #pragma unroll
@@ -445,12 +445,12 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       __syncwarp();
     };
     for (uint32_t i = 0; ok; ++i) {
-      if (!mbar_wait_warp(bar(ITEM_FULL + (i & 1)), (i >> 1) & 1, abort_flag, p.status)) break;
+      if (!mbar_wait_warp(bar(ITEM_FULL + (i & 1)), (i >> 1) & 1, abort_flag, p.status, kWaitNs)) break;
       const Item it = uniform_item(item_at(i));
       if (lane == 0) mbar_arrive(bar(ITEM_EMPTY + (i & 1)));
       if (it.last) break;
       if (it.n == 0) continue;
-      if (!mbar_wait_warp(bar(Q_FULL), nq & 1, abort_flag, p.status)) break;
+      if (!mbar_wait_warp(bar(Q_FULL), nq & 1, abort_flag, p.status, kWaitNs)) break;
       ++nq;
       const int most = seen(it, causal, min(it.q_left, it.dual ? 2 * tile_tokens : tile_tokens) - 1);
       if (it.dual) {
@@ -526,7 +526,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     float* const join_ml = reinterpret_cast<float*>(sp + Sh::kJoinMl) + row * 2;
     bool ok = true;
     for (uint32_t i = 0; ok; ++i) {
-      if (!mbar_wait_warp(bar(ITEM_FULL + (i & 1)), (i >> 1) & 1, abort_flag, p.status)) break;
+      if (!mbar_wait_warp(bar(ITEM_FULL + (i & 1)), (i >> 1) & 1, abort_flag, p.status, kWaitNs)) break;
       Item it = *item_at(i);
       it.last = (int)warp_uniform(it.last); it.n = (int)warp_uniform(it.n); it.n0 = (int)warp_uniform(it.n0);
       it.dual = (int)warp_uniform(it.dual); it.part = (int)warp_uniform(it.part);
@@ -543,7 +543,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       float m = -INFINITY, l = 0.f;          // m: the maximum that the weights are taken against
       bool first = true;
       for (int j = it.dual ? 0 : w; j < tiles; j += step) {
-        if (!mbar_wait_warp(bar(S_FULL + w), ns & 1, abort_flag, p.status)) { ok = false; break; }
+        if (!mbar_wait_warp(bar(S_FULL + w), ns & 1, abort_flag, p.status, kWaitNs)) { ok = false; break; }
         ++ns;
         if (live) {
           tc_fence_after();
@@ -629,7 +629,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       if (!ok) break;
       const bool any = (it.dual ? 0 : w) < tiles;
       if (any) {
-        if (!mbar_wait_warp(bar(O_FULL + w), no & 1, abort_flag, p.status)) break;
+        if (!mbar_wait_warp(bar(O_FULL + w), no & 1, abort_flag, p.status, kWaitNs)) break;
         ++no;
         tc_fence_after();
       }
@@ -645,7 +645,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           tmem_ld32(o_at + h * 64 + 32, o[1]);
           tmem_wait_ld(o[0]);
           tmem_wait_ld(o[1]);
-          ok = mbar_wait_warp(bar(JOIN_EMPTY + quarter), (nj & 1) ^ 1, abort_flag, p.status);
+          ok = mbar_wait_warp(bar(JOIN_EMPTY + quarter), (nj & 1) ^ 1, abort_flag, p.status, kWaitNs);
           if (!ok) break;
           ++nj;
           if (h == 0) *reinterpret_cast<float2*>(join_ml) = make_float2(m, l);
@@ -665,7 +665,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       const int64_t slot = ((int64_t)max(it.part, 0) * a.tokens_q + token) * a.heads + head;
       // rows leave through shared memory, 128 bytes of each at a time, so that a store covers 4 rows' lines and not 32
       uint8_t* const stage = sp + Sh::kJoin + quarter * 8192 + w * 4096;
-      if (w == 1 && !mbar_wait_warp(bar(JOIN_EMPTY + quarter), (nj & 1) ^ 1, abort_flag, p.status)) break;      // its own sums have been read
+      if (w == 1 && !mbar_wait_warp(bar(JOIN_EMPTY + quarter), (nj & 1) ^ 1, abort_flag, p.status, kWaitNs)) break;      // its own sums have been read
       // first token of the warp's rows; rows of 32 real queries go by one copy, others one by one
       const int slice = (quarter * 32 >> p.pack_log2) + (it.dual ? w * tile_tokens : 0);
       const bool whole = p.pack_log2 <= 5 && slice + (32 >> p.pack_log2) <= it.q_left;
@@ -684,7 +684,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           for (int e = 0; e < 64; ++e) o[e >> 5][e & 31] = 0u;
         }
         if (joined) {
-          ok = mbar_wait_warp(bar(JOIN_FULL + quarter), nj & 1, abort_flag, p.status);
+          ok = mbar_wait_warp(bar(JOIN_FULL + quarter), nj & 1, abort_flag, p.status, kWaitNs);
           if (!ok) break;
           ++nj;
           if (h == 0) {

@@ -361,7 +361,12 @@ __global__ void __launch_bounds__(256) residual_norm_rows_kernel(const __grid_co
   for (int64_t m = blockIdx.x; m < p.M; m += gridDim.x, ++i) {
     const int s = i % kSlots;
     // a wait that runs out leaves through the same barrier in every thread
-    if (__syncthreads_or(!umma::mbar_wait(smem_u32(&full[s]), (i / kSlots) & 1, &abort_flag, status))) return;
+    if (__syncthreads_or(!umma::mbar_wait(smem_u32(&full[s]), (i / kSlots) & 1, &abort_flag, status))) {
+      for (uint32_t c = i; c < i + kSlots; ++c)       // copies in flight land before the CTA leaves
+        if (m + (int64_t)(c - i) * gridDim.x < p.M)
+          for (int t = 0; t < 100000 && !umma::mbar_try_wait(smem_u32(&full[c % kSlots]), (c / kSlots) & 1); ++t) {}
+      return;
+    }
     RowReduce reduce{&red[i & 1][0][0], 8};
     in.branch = rows + used + s * 2 * K;
     in.residual = in.branch + K;

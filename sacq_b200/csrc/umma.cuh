@@ -41,15 +41,15 @@ __device__ __forceinline__ uint64_t global_timer_ns() {
   return t;
 }
 
-// Bounded wait: gives up after ~2 s or as soon as another thread of the CTA has aborted.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status) {
+// Bounded wait: gives up after ~2 s (or `limit` nanoseconds) or as soon as another thread of the CTA has aborted.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, uint64_t limit = 2000000000ull) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = global_timer_ns();
   for (uint32_t it = 0;; ++it) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((it & 63) == 63) {
       if (*abort_flag) return false;
-      if (global_timer_ns() - t0 > 2000000000ull) {
+      if (global_timer_ns() - t0 > limit) {
         *abort_flag = 1;
         atomicExch(status, kErrTimeout);
         return false;
@@ -71,8 +71,8 @@ __device__ __forceinline__ bool elect_one() {
 // A value that is the same in all lanes, marked as such.
 __device__ __forceinline__ uint32_t warp_uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 // mbar_wait by a whole converged warp, with one answer for all lanes.
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status));
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, uint64_t limit = 2000000000ull) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, limit));
 }
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
