@@ -93,8 +93,9 @@ struct AttnSplit {
 };
 __host__ __device__ __forceinline__ int key_tiles(int keys) { return (keys + kKeyTile - 1) / kKeyTile; }
 __device__ __forceinline__ int chunks_of(const AttnSplit& s, int keys) {
+  if (s.chunks_most == 1) return 1;
   const int n = (key_tiles(keys) + s.chunk - 1) / s.chunk;
-  return s.chunks_most > 1 && n > 1 ? n : 1;
+  return n > 1 ? n : 1;
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -158,8 +159,13 @@ struct ItemList {
       if (lane >= o) upto += v;
     }
   }
-  // The sequence of item `index` (not smaller than the last one asked for), and which of its items that is; false: there is none.
+  // The sequence of item `index` (best not smaller than the last one asked for), and which of its items that is; false: there is none.
   __device__ __forceinline__ bool find(int64_t index, Span& q, Span& k, int64_t& which) {
+    if (index < before) {
+      before = 0;
+      window = 0;
+      look();
+    }
     int64_t all = __shfl_sync(0xffffffffu, upto, 31);
     while (window < a.sequences && index >= before + all) {
       before += all;
@@ -179,6 +185,7 @@ struct ItemList {
 
 // The next digit of `r` in base `n`; r is left with the rest.  (A 64-bit division takes about 100 instructions.)
 __device__ __forceinline__ int digit_of(int64_t& r, int n) {
+  if (n == 1) return 0;
   if (r >> 32 == 0) {
     const uint32_t x = (uint32_t)r, y = x / (uint32_t)n;
     r = y;

@@ -4,7 +4,7 @@
 // that divides the group), so that single tokens share a tile with the other heads of their group and a causal tile's
 // diagonal is 128 / pack keys wide.  Keys come 128 at a time:
 //   S = Q K^T        tcgen05.mma, Q and K tiles in shared memory (TMA, SWIZZLE_128B), S in tensor memory, fp32
-//   P = exp(S - m)   one thread per row: running maximum and sum, no shuffles; P goes back over S as bf16
+//   P = exp(S - m)   one thread per row: running maximum and sum, no shuffles; P goes back to tensor memory as bf16
 //   O += P V         tcgen05.mma with P from tensor memory as A, the V tile as it lies (MN-major B), O in tensor memory
 // P is rounded to bf16 because V is bf16 and one instruction's operands have one type; its sum is taken before that.
 // O is rescaled only when a row's maximum has risen by more than 2^8 since the last time: until then exp(S - m) stays
@@ -12,7 +12,9 @@
 //
 // An item of work is a pair of tiles of one sequence and head group, over its keys or a chunk of them.  Both tiles
 // share the K and V tiles, each has its warpgroup, S and O: while the tensor cores work for one, the other's
-// exponentials are taken.  Where the sequence has one tile's tokens only, the two warpgroups take its keys in turn and their
+// exponentials are taken.  Up to head dim 64 P has columns of its own, and S of the next keys is made as soon as the last one is in
+// registers (8 causal prompts of 2048, 16 heads of 64: 130 against 143 us, 2 x 8192 to all keys: 684 against 791); wider, O leaves no
+// room for that, and P lies over S.  Where the sequence has one tile's tokens only, the two warpgroups take its keys in turn and their
 // results are joined.  Chunks (few items, many keys) leave fp32 results, joined by a second kernel in a fixed order.
 //
 // Roles: warps 0-3 and 4-7 softmax and epilogue of the two tiles, warp 8 MMA issuer and TMEM owner, warp 9 TMA and the
@@ -68,11 +70,12 @@ struct Shape {
   static constexpr uint32_t kItems = kBars + 8 * 64;
   static constexpr uint32_t kMisc = kItems + 2 * 64;
   static constexpr uint32_t kTotal = kMisc + 64;
-  // tensor memory columns
-  static constexpr int kS = 0, kO = 256;
+  // tensor memory columns; the weights of a wide tile lie over the first half of its S
+  static constexpr int kS = 0, kO = 256, kP = DP == 128 ? 0 : 384, kPStep = DP == 128 ? kTile : 64;
+  static constexpr bool kWide = DP == 128;
 };
 // mbarriers
-constexpr int Q_FULL = 0, Q_EMPTY = 1, S_FULL = 2, P_FULL = 4, O_FULL = 6, ITEM_FULL = 10, ITEM_EMPTY = 12,
+constexpr int Q_FULL = 0, Q_EMPTY = 1, S_FULL = 2, P_FULL = 4, O_FULL = 6, S_READ = 8, ITEM_FULL = 10, ITEM_EMPTY = 12,
               DRAIN = 14, TAKE = 15, KV_FULL = 16, KV_EMPTY = 32, JOIN_FULL = 48, JOIN_EMPTY = 52;
 
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int x, int y, int z, uint32_t src) {
@@ -252,6 +255,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     mbar_init(bar(Q_EMPTY), 1);
     for (int w = 0; w < 2; ++w) {
       mbar_init(bar(S_FULL + w), 1);
+      mbar_init(bar(S_READ + w), 4);
       mbar_init(bar(P_FULL + w), 4);
       mbar_init(bar(O_FULL + w), 1);
       mbar_init(bar(ITEM_FULL + w), 1);
@@ -334,8 +338,10 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       Span sq, sk;
       int64_t r;
       it.last = !more || !list.find(index, sq, sk, r);
-      if (more) ask();
-      if (p.dynamic && more && it.last) continue;            // there can be more items than there are: their CTAs need not begin
+      if (p.dynamic && more && it.last) {                    // there can be more items than there are: their CTAs need not begin
+        ask();
+        continue;
+      }
       if (!it.last) {
         // heads first, then chunks; the pairs of tiles from the last, longest one to the first
         const int lq = (int)sq.length, lk = (int)sk.length, chunks = chunks_of(p.split, lk);
@@ -348,7 +354,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         it.q_row = (int)sq.begin + t0;
         it.q_left = lq - t0;
         it.head = group << p.pack_log2;
-        it.kv_head = it.head / (a.heads / a.kv_heads);
+        it.kv_head = p.groups == a.kv_heads ? group : it.head / (a.heads / a.kv_heads);
         it.k_row = (int)sk.begin + first * kTile;
         it.keys = min(lk - first * kTile, n * kTile);
         it.base = lk - lq + t0 - first * kTile;
@@ -366,6 +372,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       if (lane == 0) mbar_arrive(bar(ITEM_FULL + (made & 1)));
       ++made;
       if (it.last) break;
+      ask();
       if (it.n == 0) continue;
       ok = mbar_wait_warp(bar(Q_EMPTY), (nq & 1) ^ 1, abort_flag, p.status, kWaitNs);
       if (!ok) break;
@@ -377,8 +384,8 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             tma_load_3d(sm + Sh::kQ + w * Sh::kTileBytes + h * Sh::kHalfBytes, &map_q, h * 64, it.head, it.q_row + w * tile_tokens, bar(Q_FULL));
       }
       __syncwarp();
-      // in the order of their use: K of the first step (one tile: of two), then V of a step and K of the next (next but one)
-      const int ahead = it.dual ? 1 : 2;
+      // in the order of their use: K of the first two steps (both tiles of a wide one: of one), then V of a step and the next K
+      const int ahead = it.dual && Sh::kWide ? 1 : 2;
       for (int j = 0; j < min(ahead, it.n); ++j) take(&map_k, it, j);
       for (int j = 0; j < it.n; ++j) {
         take(&map_v, it, j);
@@ -420,18 +427,16 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     // O of warpgroup w += P V over the tile's first n keys.  (What the instructions are issued with has to be in uniform
     // registers, and the warp converged in front of and behind each group: 120 clocks each otherwise, 64 so.)
     auto pv = [&](int w, uint32_t s, int n, bool first) {
+      if (!ok) return;
       n = (int)warp_uniform(n); w = (int)warp_uniform(w); s = warp_uniform(s);
       const uint64_t vd = make_mn_desc(sm + Sh::kRing + s * Sh::kTileBytes, Sh::kHalfBytes);
       const uint32_t more = warp_uniform(first ? 0u : 1u);
-      ok = ok && mbar_wait_warp(bar(P_FULL + w), (w == 0 ? np0 : np1) & 1, abort_flag, p.status, kWaitNs);
-      if (!ok) return;
       tc_fence_after();
 #pragma unroll
       for (int i = 0; i < kTile / 16; ++i)
         if (i * 16 < n && elect_one())
-          umma_bf16_ts(tmem + Sh::kO + w * DP, tmem + Sh::kS + w * kTile + i * 8, vd + (uint64_t)(i * 2048 >> 4), idesc_pv, i > 0 ? 1u : more);
+          umma_bf16_ts(tmem + Sh::kO + w * DP, tmem + Sh::kP + w * Sh::kPStep + i * 8, vd + (uint64_t)(i * 2048 >> 4), idesc_pv, i > 0 ? 1u : more);
       __syncwarp();
-      if (w == 0) ++np0; else ++np1;
     };
     // rows of a V tile behind the last key, up to a whole instruction: zeros, whatever lies there in memory
     auto clear_tail = [&](uint32_t s, int keys) {
@@ -455,60 +460,83 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       const int most = seen(it, causal, min(it.q_left, it.dual ? 2 * tile_tokens : tile_tokens) - 1);
       if (it.dual) {
         const int most0 = seen(it, causal, tile_tokens - 1);
+        auto scores = [&](int w, int j, uint32_t ks) {
+          qk(w, w, ks, columns(w == 0 ? most0 : most, j));
+          commit(S_FULL + w);
+        };
+        auto arrived = [&](int b, uint32_t phase) { ok = ok && mbar_wait_warp(bar(b), phase & 1, abort_flag, p.status, kWaitNs); };
         uint32_t ks = next();
-        if (it.n0 > 0) {
-          qk(0, 0, ks, columns(most0, 0));
-          commit(S_FULL + 0);
-        }
-        qk(1, 1, ks, columns(most, 0));
-        commit(S_FULL + 1);
+        if (it.n0 > 0) scores(0, 0, ks);
+        scores(1, 0, ks);
         commit(KV_EMPTY + ks);
         if (it.n == 1) commit(Q_EMPTY);
         for (int j = 0; j < it.n && ok; ++j) {
-          const uint32_t vs = next();
-          clear_tail(vs, it.keys - j * kTile);
-          if (j < it.n0) pv(0, vs, columns(most0, j), j == 0);
-          if (j + 1 < it.n) ks = next();
-          if (j + 1 < it.n0) {
-            qk(0, 0, ks, columns(most0, j + 1));
-            commit(S_FULL + 0);
-          } else if (j + 1 == it.n0) {
-            commit(O_FULL + 0);
-          }
-          pv(1, vs, columns(most, j), j == 0);
-          commit(KV_EMPTY + vs);
-          if (j + 1 < it.n) {
-            qk(1, 1, ks, columns(most, j + 1));
-            commit(S_FULL + 1);
-            commit(KV_EMPTY + ks);
-            if (j + 2 == it.n) commit(Q_EMPTY);
-          } else {
+          if constexpr (!Sh::kWide) {        // S of the next keys as soon as the last one is in registers, beside the exponentials
+            if (j + 1 < it.n) {
+              ks = next();
+              if (j + 1 < it.n0) {
+                arrived(S_READ + 0, np0);
+                tc_fence_after();
+                scores(0, j + 1, ks);
+              }
+              arrived(S_READ + 1, np1);
+              tc_fence_after();
+              scores(1, j + 1, ks);
+              commit(KV_EMPTY + ks);
+              if (j + 2 == it.n) commit(Q_EMPTY);
+            }
+            const uint32_t vs = next();
+            clear_tail(vs, it.keys - j * kTile);
+            if (j < it.n0) {
+              arrived(P_FULL + 0, np0++);
+              pv(0, vs, columns(most0, j), j == 0);
+              commit(O_FULL + 0);
+            }
+            arrived(P_FULL + 1, np1++);
+            pv(1, vs, columns(most, j), j == 0);
             commit(O_FULL + 1);
+            commit(KV_EMPTY + vs);
+          } else {                           // the weights lie over S: it is made behind P V
+            const uint32_t vs = next();
+            clear_tail(vs, it.keys - j * kTile);
+            if (j < it.n0) {
+              arrived(P_FULL + 0, np0++);
+              pv(0, vs, columns(most0, j), j == 0);
+            }
+            if (j + 1 < it.n) ks = next();
+            if (j + 1 < it.n0) scores(0, j + 1, ks);
+            else if (j + 1 == it.n0) commit(O_FULL + 0);
+            arrived(P_FULL + 1, np1++);
+            pv(1, vs, columns(most, j), j == 0);
+            commit(KV_EMPTY + vs);
+            if (j + 1 < it.n) {
+              scores(1, j + 1, ks);
+              commit(KV_EMPTY + ks);
+              if (j + 2 == it.n) commit(Q_EMPTY);
+            } else {
+              commit(O_FULL + 1);
+            }
           }
         }
       } else {
-        for (int j = 0; j < min(2, it.n); ++j) {
+        auto scores = [&](int w, int j) {
           const uint32_t ks = next();
-          qk(j, 0, ks, columns(most, j));
-          commit(S_FULL + j);
+          qk(w, 0, ks, columns(most, j));
+          commit(S_FULL + w);
           commit(KV_EMPTY + ks);
-        }
-        if (it.n <= 2) commit(Q_EMPTY);
+          if (j + 1 == it.n) commit(Q_EMPTY);
+        };
+        for (int j = 0; j < min(2, it.n); ++j) scores(j, j);
         for (int j = 0; j < it.n && ok; ++j) {
           const int w = j & 1;
           const uint32_t vs = next();
           clear_tail(vs, it.keys - j * kTile);
+          ok = ok && mbar_wait_warp(bar(P_FULL + w), (w == 0 ? np0 : np1) & 1, abort_flag, p.status, kWaitNs);
           pv(w, vs, columns(most, j), j < 2);
+          if (w == 0) ++np0; else ++np1;
+          if (!Sh::kWide || j + 2 >= it.n) commit(O_FULL + w);
           commit(KV_EMPTY + vs);
-          if (j + 2 < it.n) {
-            const uint32_t ks = next();
-            qk(w, 0, ks, columns(most, j + 2));
-            commit(S_FULL + w);
-            commit(KV_EMPTY + ks);
-            if (j + 3 == it.n) commit(Q_EMPTY);
-          } else {
-            commit(O_FULL + w);
-          }
+          if (j + 2 < it.n) scores(w, j + 2);
         }
       }
     }
@@ -519,7 +547,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     const int w = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const uint32_t s_at = tmem + lanes + Sh::kS + w * kTile, o_at = tmem + lanes + Sh::kO + w * DP;
+    const uint32_t s_at = tmem + lanes + Sh::kS + w * kTile, p_at = tmem + lanes + Sh::kP + w * Sh::kPStep, o_at = tmem + lanes + Sh::kO + w * DP;
     const float c2 = a.scale * kLog2e;
     uint32_t ns = 0, no = 0, nj = 0;         // steps, items with keys, halves joined
     float* const join = reinterpret_cast<float*>(sp + Sh::kJoin) + row * 64;
@@ -533,7 +561,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       if (lane == 0) mbar_arrive(bar(ITEM_EMPTY + (i & 1)));
       if (it.last) break;
       // this warp's copies out have read their room: where a lone tile's sums will be handed over
-      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      if (!it.dual && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       const int t = (row >> p.pack_log2) + (it.dual ? w * tile_tokens : 0);      // token of the item
       const bool valid = t < it.q_left;
       const bool live = __any_sync(0xffffffffu, valid);
@@ -563,6 +591,11 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             } else {
               tmem_wait_ld(s[2]);
               tmem_wait_ld(s[3]);
+              if (!Sh::kWide) {              // S may be made anew
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(S_READ + w));
+              }
             }
             if (masked) {                    // columns that this row does not see
 #pragma unroll
@@ -581,6 +614,11 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 top[b & 1] = max_nan(top[b & 1], __uint_as_float(s[b][e]), __uint_as_float(s[b][e + 1]));
           }
           const float high = max_nan(top[0], top[1], top[1]);
+          if (!Sh::kWide && j >= step) {     // O and P of the step before are done with (wide: known from S)
+            ok = mbar_wait_warp(bar(O_FULL + w), no & 1, abort_flag, p.status, kWaitNs);
+            ++no;
+            tc_fence_after();
+          }
           if (__any_sync(0xffffffffu, !((high - m) * c2 <= kRescale))) {      // NaN: yes
             const float keep = m == -INFINITY ? 0.f : exp2_fast((m - high) * c2);
             m = high;
@@ -614,14 +652,21 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
               sum[e & 1] = add2(sum[e & 1], w2);
               weights[e] = bf16_pair(x, y);
             }
-            tmem_st32(s_at + h * 32, weights);
+            tmem_st32(p_at + h * 32, weights);
           }
           float x, y;
           halves_of(add2(sum[0], sum[1]), x, y);
           l += x + y;
           tmem_wait_st();
           first = false;
+        } else {
+          if (!Sh::kWide && lane == 0) mbar_arrive(bar(S_READ + w));
+          if (!Sh::kWide && j >= step) {
+            ok = ok && mbar_wait_warp(bar(O_FULL + w), no & 1, abort_flag, p.status, kWaitNs);
+            ++no;
+          }
         }
+        if (!ok) break;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(P_FULL + w));
