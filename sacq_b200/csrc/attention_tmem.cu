@@ -600,6 +600,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             if (masked) {                    // columns that this row does not see
 #pragma unroll
               for (int b = 2 * h; b < 2 * h + 2; ++b) {
+                if (Sh::kWide && (b + 1) * 32 <= least - j * kTile) continue;      // (narrow: 131 us became 137)
                 const int left = end - b * 32;
                 const uint32_t visible = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
 #pragma unroll
