@@ -417,6 +417,19 @@ def test_residual_norm_vectors_of_each_request(m):
     assert torch.equal(got[0][clean], keep[0][clean]) and bool(got[0][~clean].isnan().all()) and bool(got[1][~clean].isnan().all())
 
 
+@pytest.mark.parametrize("m,k", ((9001, 8), (3000, 256), (4500, 520), (2500, 768), (2000, 1000), (1800, 1792), (2700, 2048), (1200, 2056), (1100, 8192)))
+@pytest.mark.parametrize("vectors", (0, 7))
+def test_residual_norm_of_many_rows(m, k, vectors):
+    """Each width of the kernels for many rows, several rows after another, with and without tables."""
+    from sacq_b200 import residual_norm_quantize_rows
+    for norm, post, modulated, affine in (("rms", "rms", False, True), ("rms", None, False, False), ("layer", "layer", True, True)):
+        branch, residual, p, rows, ref = _norm_case(m, k, norm, post, vectors, seed=m + k, modulated=modulated, affine=affine)
+        got = residual_norm_quantize_rows(branch, residual, p["weight"], p["bias"], norm=norm, post_norm=post, post_weight=p["post_weight"],
+                                          post_bias=p["post_bias"], gate=p["gate"], mod_scale=p["mod_scale"], mod_shift=p["mod_shift"],
+                                          vector_rows=rows)
+        _check_norm(got, ref)
+
+
 def test_residual_norm_without_vectors_zeros_and_what_is_not_finite():
     from sacq_b200 import residual_norm_quantize_rows
     for m in (4, 1200):
