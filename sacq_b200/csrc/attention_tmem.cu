@@ -753,6 +753,10 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           }
           __syncwarp();
         }
+        if (h * 64 + 64 > a.dim)             // columns of tensor memory that no product writes may hold anything
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (h * 64 + e >= a.dim) o[e >> 5][e & 31] = 0u;
         if (h == 0) inv = mine > 0 ? 1.0f / l : 0.f;
         const uint64_t inv2 = f32x2(inv, inv);
         uint64_t odd2 = f32x2(0.f, 0.f);     // NaN if a value is not finite
