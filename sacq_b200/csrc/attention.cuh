@@ -201,8 +201,8 @@ int launch_attention_join(const AttnParams& a, const AttnSplit& split, cudaStrea
 
 // Head dims that are multiples of 8 up to 128, rows that TMA can read.
 bool attention_tma_supported(const AttnParams& p);
-// How a call is cut up for a kernel with `slots` CTAs at once: `items` pieces of work without a cut.
-AttnSplit attention_split(const AttnParams& a, int64_t items, int64_t items_per_sequence, int64_t slots, int min_chunk, void* workspace);
+// A call in chunks of `chunk` key tiles, or of more where their results would not fit 256 MB; 0: not cut up.
+AttnSplit attention_chunks(const AttnParams& a, int64_t chunk, void* workspace);
 int64_t attention_split_bytes(const AttnParams& a, const AttnSplit& split);
 int attention_tensor_maps(const AttnParams& a, int q_box_heads, int q_box_tokens, int k_box_tokens, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v);
 int attention_out_map(const AttnParams& a, int box_heads, int box_tokens, CUtensorMap* out);

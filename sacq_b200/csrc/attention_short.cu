@@ -395,10 +395,17 @@ int64_t short_items(const AttnParams& a, int64_t* per_sequence) {
 
 }  // namespace
 
+// Only the sizes of a call are known here, not its offsets.  It is cut where it has fewer than four items for each CTA: into a
+// quarter of a CTA's share each, if the sequences are alike; a chunk's start and its part in the join would outweigh less than 4 tiles.
 AttnSplit attention_short_split(const AttnParams& a, void* workspace) {
   int64_t per_sequence = 0;
-  const int64_t items = short_items(a, &per_sequence);
-  return attention_split(a, items, per_sequence, 2 * device_sms() * 3 / 4, 4, workspace);
+  const int64_t items = short_items(a, &per_sequence), slots = 2 * device_sms() * 3 / 4, tiles = (a.tokens_k + kKeyTile - 1) / kKeyTile;
+  int64_t chunk = 0;
+  if (items < 4 * slots) {
+    chunk = (tiles + a.sequences) * per_sequence / (4 * slots);
+    if (chunk < 4) chunk = 4;
+  }
+  return attention_chunks(a, chunk, workspace);
 }
 
 int launch_attention_short(const AttnParams& a, const AttnSplit& split, cudaStream_t s) {

@@ -110,16 +110,12 @@ bool attention_tma_supported(const AttnParams& a) {
          strides_for_tma(a.k_token, a.k_head, a.kv_heads, a.tokens_k) && strides_for_tma(a.v_token, a.v_head, a.kv_heads, a.tokens_k);
 }
 
-// Only the sizes of a call are known here, not its offsets.  It is cut where it has fewer than four items for each CTA: into a
-// quarter of a CTA's share each, if the sequences are alike.
-AttnSplit attention_split(const AttnParams& a, int64_t items, int64_t items_per_sequence, int64_t slots, int min_chunk, void* workspace) {
+AttnSplit attention_chunks(const AttnParams& a, int64_t chunk, void* workspace) {
   AttnSplit s = {};
   const int64_t tiles = (a.tokens_k + kKeyTile - 1) / kKeyTile;            // of the longest sequence there can be
   s.chunk = (int)(tiles < 1 ? 1 : tiles);
   s.chunks_most = 1;
-  if (items < 4 * slots) {
-    int64_t chunk = (tiles + a.sequences) * items_per_sequence / (4 * slots);
-    if (chunk < min_chunk) chunk = min_chunk;                              // a chunk's start and its part in the join would outweigh less
+  if (chunk > 0) {
     const int64_t most_bytes = 256ll << 20, row = a.tokens_q * a.heads * (a.dim + 1) * 4;
     while (chunk < tiles && (tiles + chunk - 1) / chunk * row > most_bytes) chunk *= 2;
     if (2 * chunk <= tiles + 1) {

@@ -805,12 +805,23 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 *reinterpret_cast<uint4*>(a.out + ((int64_t)it.q_row + tt) * a.out_token + (int64_t)(it.head + (rr & ((1 << p.pack_log2) - 1))) * a.out_head + d) = v;
             }
           }
-        } else if (valid) {
-          float* const po = p.split.part_o + slot * a.dim + h * 64;
+        } else {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const uint32_t* const u = &o[e >> 3][4 * (e & 7)];
-            if (h * 64 + e * 4 < a.dim) *reinterpret_cast<uint4*>(po + e * 4) = make_uint4(u[0], u[1], u[2], u[3]);
+          for (int g = 0; g < 2; ++g) {      // fp32: 32 columns of 32 rows at a time
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ (lane & 7)) << 4)) = make_uint4(o[g][4 * e], o[g][4 * e + 1], o[g][4 * e + 2], o[g][4 * e + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int r = e * 4 + (lane >> 3), piece = lane & 7, rr = quarter * 32 + r;
+              const int tt = (rr >> p.pack_log2) + (it.dual ? w * tile_tokens : 0), d = h * 64 + g * 32 + piece * 4;
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((piece ^ (r & 7)) << 4));
+              if (tt < it.q_left && d < a.dim)
+                *reinterpret_cast<uint4*>(p.split.part_o + (((int64_t)it.part * a.tokens_q + it.q_row + tt) * a.heads + it.head + (rr & ((1 << p.pack_log2) - 1))) * a.dim + d) = v;
+            }
           }
         }
         __syncwarp();
@@ -869,9 +880,27 @@ Tiles tiles_of(const AttnParams& a) {
 
 }  // namespace
 
+// Cutting keys up costs a second kernel and fp32 parts that are written and read (the longest item of a call is shorter then, nothing
+// else): 9 us and 8 bytes an element and part at 5 TB/s.  A step of 128 keys takes 0.9 us, of two tiles 2.  Measured, without and with
+// chunks of 8 tiles: 1 x 64 queries to 16,384 keys, 16 / 8 heads, 118 and 27 us; 4 x 100 to 4,000, 8 heads, 37 and 24; 8 x 33 to
+// 2,000, 16 / 8 heads, 23 and 24; prompts of 2,048, 16 / 8 heads, 37 and 64; 2,517, 12 heads, 45 and 82.
 AttnSplit attention_tmem_split(const AttnParams& a, void* workspace) {
   const Tiles t = tiles_of(a);
-  return attention_split(a, t.items, t.per_sequence, device_sms(), 4, workspace);
+  const double tiles = (double)((a.tokens_k + kKeyTile - 1) / kKeyTile), average = ceil(tiles / a.sequences);
+  const double longest = a.sequences == 1 ? tiles : fmin(tiles, 2 * average);
+  const bool pairs = a.tokens_q > (int64_t)a.sequences * (kTile >> t.pack_log2), half = a.causal && 2 * a.tokens_q > a.tokens_k;
+  const double step = pairs ? 2.0 : 0.9, share = (double)t.items * average * (half ? 0.5 : 1.0) / device_sms();
+  const double part = (double)a.tokens_q * a.heads * a.dim * 8 / 5e6;
+  double best = 0.85 * step * fmax(longest, share);
+  int64_t chunk = 0;
+  for (int64_t c = 8; c < longest; c *= 2) {
+    const double us = step * fmax((double)c, share) + 9 + part * ceil(average / (double)c);
+    if (us < best) {
+      best = us;
+      chunk = c;
+    }
+  }
+  return attention_chunks(a, chunk, workspace);
 }
 
 int launch_attention_tmem(const AttnParams& a, const AttnSplit& split, cudaStream_t s) {
