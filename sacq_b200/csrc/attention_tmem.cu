@@ -228,7 +228,8 @@ __device__ __forceinline__ int seen(const Item& it, bool causal, int t) { return
 // Columns of key tile j that the tile's last token sees, in whole instructions of 16.
 __device__ __forceinline__ int columns(int most, int j) { return (min(kTile, most - j * kTile) + 15) & ~15; }
 
-template <int DP>
+// SPLIT: there may be chunks (their code costs the others registers: 44.6 us of the 64 x 256 tokens became 47.3).
+template <int DP, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o,
@@ -344,7 +345,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       }
       if (!it.last) {
         // heads first, then chunks; the pairs of tiles from the last, longest one to the first
-        const int lq = (int)sq.length, lk = (int)sk.length, chunks = chunks_of(p.split, lk);
+        const int lq = (int)sq.length, lk = (int)sk.length, chunks = SPLIT ? chunks_of(p.split, lk) : 1;
         const int pairs = (lq + 2 * tile_tokens - 1) >> (tokens_log2 + 1);
         const int group = digit_of(r, p.groups), part = digit_of(r, chunks);
         const int pair = pairs - 1 - (int)r;
@@ -778,7 +779,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 #pragma unroll
           for (int e = 0; e < 64; ++e) o[e >> 5][e & 31] = 0u;
         }
-        if (it.part < 0) {
+        if (!SPLIT || it.part < 0) {
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");    // the last copy from here has read it
           __syncwarp();
 #pragma unroll
@@ -805,7 +806,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 *reinterpret_cast<uint4*>(a.out + ((int64_t)it.q_row + tt) * a.out_token + (int64_t)(it.head + (rr & ((1 << p.pack_log2) - 1))) * a.out_head + d) = v;
             }
           }
-        } else {
+        } else if constexpr (SPLIT) {
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 #pragma unroll
           for (int g = 0; g < 2; ++g) {      // fp32: 32 columns of 32 rows at a time
@@ -833,7 +834,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       if (!ok) break;
       if (valid) {
         const float le = mine > 0 ? fmaf(m, a.scale, log2_fast(l) * 0.693147180559945f) : -INFINITY;
-        if (it.part >= 0) p.split.part_lse[slot] = le;
+        if (SPLIT && it.part >= 0) p.split.part_lse[slot] = le;
         else if (a.lse != nullptr) a.lse[token * a.heads + head] = le;
       }
       // a value that is not finite may have come in with a weight of zero: from keys that other rows of the tile see, or
@@ -849,7 +850,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       while (odd != 0) {
         const int src = __ffs(odd) - 1;
         odd &= odd - 1;
-        redo_row(a, p.split, it.k_row, it.kv_head, it.part, __shfl_sync(0xffffffffu, token, src), __shfl_sync(0xffffffffu, head, src),
+        redo_row(a, p.split, it.k_row, it.kv_head, SPLIT ? it.part : -1, __shfl_sync(0xffffffffu, token, src), __shfl_sync(0xffffffffu, head, src),
                  __shfl_sync(0xffffffffu, mine, src), 0, DP);
       }
     }
@@ -918,14 +919,16 @@ int launch_attention_tmem(const AttnParams& a, const AttnSplit& split, cudaStrea
   if (int rc = attention_tensor_maps(a, pack, kTile / pack, kTile, &mq, &mk, &mv)) return rc;
   if (int rc = attention_out_map(a, pack < 32 ? pack : 32, pack < 32 ? 32 / pack : 1, &mo)) return rc;
   const bool wide = a.dim > 64;
-  const void* fn = wide ? (const void*)attention_tmem_kernel<128> : (const void*)attention_tmem_kernel<64>;
+  const bool cut = split.chunks_most > 1;
+  const void* fn = wide ? (cut ? (const void*)attention_tmem_kernel<128, true> : (const void*)attention_tmem_kernel<128, false>)
+                        : (cut ? (const void*)attention_tmem_kernel<64, true> : (const void*)attention_tmem_kernel<64, false>);
   const size_t smem = (wide ? Shape<128>::kTotal : Shape<64>::kTotal) + 1024;
-  static bool configured[2][64] = {};
+  static bool configured[2][2][64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !configured[wide][dev]) {
+  if (dev < 0 || dev >= 64 || !configured[wide][cut][dev]) {
     SACQ_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    if (dev >= 0 && dev < 64) configured[wide][dev] = true;
+    if (dev >= 0 && dev < 64) configured[wide][cut][dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
   // Items differ in length (a causal prompt's last tile has all its keys): CTAs that take the next one when they are done
