@@ -112,6 +112,32 @@ def test_attention_to_keys_of_other_lengths(lq, lk, causal):
     _attend(lq, lk, 3, 3, 64, causal, seed=1)
 
 
+@pytest.mark.parametrize("lq,lk,heads,kv_heads", (([100, 100], [4000, 3001], 4, 4), ([130], [6000], 2, 2), ([300, 3], [5100, 129], 3, 1), ([70, 1, 65], [5000, 0, 140], 4, 2),
+                                                  ([2300], [2300], 1, 1), ([5, 1], [7000, 200], 4, 2)))
+@pytest.mark.parametrize("dim", (128, 64, 80, 40))
+@pytest.mark.parametrize("causal", (False, True))
+def test_attention_of_few_queries_to_many_keys(lq, lk, heads, kv_heads, dim, causal):
+    """Keys in chunks of several tiles, one and two tiles of queries; rows that a chunk holds nothing for."""
+    _attend(lq, lk, heads, kv_heads, dim, causal, seed=7)
+
+
+@pytest.mark.parametrize("dim", (128, 64))
+def test_attention_of_chunks_keeps_what_is_not_seen_out(dim):
+    from sacq_b200 import attention_packed
+    gen = _gen(9)
+    q, (k, v) = _randn(gen, 90, 2, dim), (_randn(gen, 5000, 2, dim) for _ in range(2))
+    cu_q, cu_k = _offsets([90]), _offsets([4700])
+    want = attention_packed(q, k, v, cu_q, cu_k, causal=True, return_lse=True)
+    for t in (k, v):
+        t[4700:] = NAN
+        t[4690:4700] = INF                   # seen by the last queries only
+    got = attention_packed(q, k, v, cu_q, cu_k, causal=True, return_lse=True)
+    # rows that see none of them are made again key by key there: other roundings of the same sums
+    assert float((got[0][:80].double() - want[0][:80].double()).abs().max()) <= 2 * BF * float(want[0].abs().max())
+    assert float((got[1][:80] - want[1][:80]).abs().max()) <= 2 * 4700 * F32          # two fp32 sums of as many weights
+    assert not bool(torch.isfinite(got[0][80:].float()).all(dim=-1).any())
+
+
 def test_attention_of_many_sequences():
     lengths = [(7 * i) % 40 for i in range(300)]
     _attend(lengths, lengths, 2, 1, 64, True)
