@@ -31,6 +31,28 @@ __device__ __forceinline__ Span span_of(const int32_t* cu, int s, int64_t tokens
   return {a, b > a ? b - a : 0};
 }
 
+// The sequence that a query token lies in, by a whole warp; -1: none.  Offsets that never go down are bisected, in which the last sequence that
+// begins at or in front of the token is found; where that one does not hold it, because sequences lie in another order, empty ones
+// begin in front of it, or none does, all are looked at, 32 at a time.
+__device__ __forceinline__ int sequence_of(const int32_t* cu_q, int sequences, int64_t tokens_q, int64_t token) {
+  auto holds = [&](int s) {
+    const Span q = span_of(cu_q, s, tokens_q);
+    return token >= q.begin && token < q.begin + q.length;
+  };
+  int lo = 0, hi = sequences;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu_q[mid] <= token) lo = mid; else hi = mid;
+  }
+  if (holds(lo)) return lo;
+  for (int first = 0; first < sequences; first += 32) {
+    const int s = first + (threadIdx.x & 31);
+    const uint32_t found = __ballot_sync(0xffffffffu, s < sequences && holds(s));
+    if (found != 0) return first + __ffs(found) - 1;
+  }
+  return -1;
+}
+
 // One query row by one warp, key after key with a running maximum: lane l holds elements l, l + 32, ...  Returns the
 // row's 1 / sum and leaves the sums in acc.
 template <int E>

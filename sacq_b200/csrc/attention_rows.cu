@@ -17,15 +17,9 @@ __global__ void __launch_bounds__(kRowWarps * 32) attention_rows_kernel(const __
   const int64_t token = item / p.heads;
   const int head = (int)(item - token * p.heads);
   if (token >= p.tokens_q) return;
-  // the sequence that holds the token: the last one that begins at or in front of it
-  int lo = 0, hi = p.sequences;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.cu_q[mid] <= token) lo = mid; else hi = mid;
-  }
-  const Span sq = span_of(p.cu_q, lo, p.tokens_q);
-  if (token < sq.begin || token >= sq.begin + sq.length) return;      // in front of the first sequence or behind the last
-  const Span sk = span_of(p.cu_k, lo, p.tokens_k);
+  const int sequence = sequence_of(p.cu_q, p.sequences, p.tokens_q, token);
+  if (sequence < 0) return;
+  const Span sq = span_of(p.cu_q, sequence, p.tokens_q), sk = span_of(p.cu_k, sequence, p.tokens_k);
   int64_t keys = sk.length;
   if (p.causal) keys = min(keys, max((int64_t)0, token - sq.begin + 1 + sk.length - sq.length));
   const int kv = head / (p.heads / p.kv_heads);

@@ -17,14 +17,9 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
   const int64_t token = item / a.heads;
   const int head = (int)(item - token * a.heads);
   if (token >= a.tokens_q) return;
-  int lo = 0, hi = a.sequences;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu_q[mid] <= token) lo = mid; else hi = mid;
-  }
-  const Span sq = span_of(a.cu_q, lo, a.tokens_q);
-  if (token < sq.begin || token >= sq.begin + sq.length) return;
-  const Span sk = span_of(a.cu_k, lo, a.tokens_k);
+  const int sequence = sequence_of(a.cu_q, a.sequences, a.tokens_q, token);
+  if (sequence < 0) return;
+  const Span sk = span_of(a.cu_k, sequence, a.tokens_k);
   const int chunks = chunks_of(split, (int)sk.length);
   if (chunks == 1) return;                   // written by the attention kernel
   const int64_t stride = a.tokens_q * a.heads, at = token * a.heads + head;

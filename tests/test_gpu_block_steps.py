@@ -724,6 +724,51 @@ print("same")
     assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
 
 
+def _cut_up(q, k, v, cu_q, cu_k, causal=False):
+    """Whether the call's keys go in chunks: it needs room for their results."""
+    import ctypes
+    from sacq_b200 import _lib
+    d = _lib.AttentionDesc(struct_size=ctypes.sizeof(_lib.AttentionDesc), causal=causal, q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=q.data_ptr(),
+                           tokens_q=q.shape[0], tokens_k=k.shape[0], cu_q=cu_q.data_ptr(), cu_k=cu_k.data_ptr(), sequences=cu_q.numel() - 1,
+                           heads=q.shape[1], kv_heads=k.shape[1], head_dim=q.shape[2], scale=1.0)
+    for n, t in (("q", q), ("k", k), ("v", v), ("out", q)):
+        setattr(d, n + "_token", t.stride(0))
+        setattr(d, n + "_head", t.stride(1))
+    return _lib.load().sacq_attention_workspace_bytes(ctypes.byref(d)) > 0
+
+
+@pytest.mark.parametrize("cu_q,cu_k,heads,kv_heads,dim,cut", (
+    ([0, 1, 2, 0, 0, 0, 0, 0, 0], [0, 9000, 18000, 0, 0, 0, 0, 0, 0], 4, 2, 128, True),                  # 16-row tiles
+    ([0, 100, 200, 0, 0, 0, 0, 0, 0], [0, 9000, 18000, 0, 0, 0, 0, 0, 0], 4, 2, 64, True),               # 128-row tiles
+    ([40, 60, 20, 30, 0, 15], [2000, 9000, 1000, 2000, 0, 1000], 2, 2, 64, True),
+    ([40, 60, 20, 30, 0, 15], [2000, 9000, 1000, 2000, 0, 1000], 8, 1, 128, True),
+    ([0, 10, 50, 0, 0, 0, 0, 0], [0, 10, 50, 0, 0, 0, 0, 0], 2, 1, 36, False),                           # a warp per row
+    ([40, 60, 20, 30, 0, 15], [200, 900, 100, 200, 0, 100], 2, 1, 36, False),
+    ([0, 10, 50, 0, 0, 0, 0, 0], [0, 10, 50, 0, 0, 0, 0, 0], 2, 1, 64, False),
+    ([0] * 70 + [3, 8] + [0] * 70, [0] * 70 + [40, 60] + [0] * 70, 2, 1, 36, False)))
+@pytest.mark.parametrize("causal", (False, True))
+def test_attention_of_offsets_that_go_down(cu_q, cu_k, heads, kv_heads, dim, cut, causal):
+    """Sequences in any order, empty ones anywhere: each row of a sequence is made by every kernel, and no other row is touched."""
+    from sacq_b200 import attention_packed
+    gen = _gen(11)
+    spans = [(a, max(b - a, 0), c, max(d - c, 0)) for a, b, c, d in zip(cu_q, cu_q[1:], cu_k, cu_k[1:])]
+    tokens_q, tokens_k = max(cu_q) + 5, max(cu_k) + 5
+    q = _randn(gen, tokens_q, heads, dim, by=1.5)
+    k, v = (_randn(gen, tokens_k, kv_heads, dim, by=1.5) for _ in range(2))
+    offsets = [torch.tensor(c, dtype=torch.int32, device="cuda") for c in (cu_q, cu_k)]
+    assert _cut_up(q, k, v, *offsets, causal) == cut
+    out = torch.full_like(q, 3.0)
+    lse = attention_packed(q, k, v, *offsets, causal=causal, out=out, return_lse=True)[1]
+    left = torch.ones(tokens_q, dtype=torch.bool, device="cuda")
+    for at_q, nq, at_k, nk in spans:
+        if nq == 0:
+            continue
+        rows, keys = slice(at_q, at_q + nq), slice(at_k, at_k + nk)
+        _check_attention(out[rows], lse[rows], _attention_reference(q[rows], k[keys], v[keys], [nq], [nk], causal))
+        left[rows] = False
+    assert bool((out[left] == 3).all())
+
+
 def test_no_wait_has_run_out():
     import ctypes
     from sacq_b200 import _lib
