@@ -348,7 +348,7 @@ attention_short_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       if (!ok) break;
     }
     if (warp >= 2) continue;
-    uint32_t odd = 0;                        // rows with a value that is not finite and keys that others of the tile see
+    uint32_t odd = 0;                        // rows with a value that is not finite and keys among those multiplied that they do not see
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float inv = mine[h] > 0 ? 1.0f / l[h] : 0.f;
@@ -370,7 +370,8 @@ attention_short_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         if (it.part >= 0) p.split.part_lse[slot] = le;
         else if (a.lse != nullptr) a.lse[(int64_t)token[h] * a.heads + head[h]] = le;
       }
-      const uint32_t bad = __ballot_sync(0xffffffffu, valid[h] && !finite && mine[h] > 0 && mine[h] < min((most + 15) & ~15, it.keys));
+      // a warp multiplies 32 keys at a time, those of the last 32 that no row of the tile sees among them
+      const uint32_t bad = __ballot_sync(0xffffffffu, valid[h] && !finite && mine[h] > 0 && mine[h] < min((most + 31) & ~31, it.keys));
 #pragma unroll
       for (int r = 0; r < 8; ++r)
         if (bad & (0xfu << (4 * r))) odd |= 1u << (r + 8 * h);

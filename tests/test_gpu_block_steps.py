@@ -769,6 +769,46 @@ def test_attention_of_offsets_that_go_down(cu_q, cu_k, heads, kv_heads, dim, cut
     assert bool((out[left] == 3).all())
 
 
+@pytest.mark.parametrize("lq,past,heads,kv_heads,dim", ((32, 0, 1, 1, 64), (27, 0, 2, 2, 128), (17, 0, 1, 1, 40), (16, 8, 2, 1, 128), (16, 30, 4, 2, 64), (9, 23, 3, 1, 96),
+                                                        (3, 0, 2, 1, 64), (16, 7001, 2, 1, 128), (30, 9020, 1, 1, 64), (16, 90, 2, 1, 72)))
+@pytest.mark.parametrize("value", (NAN, INF))
+def test_attention_of_few_queries_keeps_later_keys_out(value, lq, past, heads, kv_heads, dim):
+    """16-row tiles: for every token, all keys behind those that it sees hold anything."""
+    from sacq_b200 import attention_packed
+    gen = _gen(12)
+    n = past + lq
+    q, k, v = _randn(gen, lq, heads, dim), _randn(gen, n, kv_heads, dim), _randn(gen, n, kv_heads, dim)
+    cu_q, cu_k = _offsets([lq]), _offsets([n])
+    assert lq * (heads // kv_heads) <= 32 and _cut_up(q, k, v, cu_q, cu_k, True) == (past > 5000)
+    ref = _attention_reference(q, k, v, [lq], [n], True)
+    for t in range(lq):
+        k2, v2 = k.clone(), v.clone()
+        k2[past + t + 1:], v2[past + t + 1:] = value, value
+        got, lse = attention_packed(q, k2, v2, cu_q, cu_k, causal=True, return_lse=True)
+        _check_attention(got[:t + 1], lse[:t + 1], tuple(x[:t + 1] for x in ref))
+
+
+@pytest.mark.parametrize("lq,lk", (([5, 16, 2], [37, 70, 61]), ([1, 1, 1], [200, 16, 33]), ([4, 9, 1], [9000, 7, 50])))
+@pytest.mark.parametrize("heads,kv_heads,dim", ((2, 1, 128), (2, 2, 64), (3, 1, 24)))
+@pytest.mark.parametrize("value", (NAN, -INF))
+def test_attention_of_few_queries_keeps_other_sequences_out(value, heads, kv_heads, dim, lq, lk):
+    from sacq_b200 import attention_packed
+    gen = _gen(13)
+    q = _randn(gen, sum(lq) + 6, heads, dim)
+    k, v = (_randn(gen, sum(lk) + 6, kv_heads, dim) for _ in range(2))
+    cu_q, cu_k = _offsets(lq) + 3, _offsets(lk) + 3
+    at_q = at_k = 3
+    for nq, nk in zip(lq, lk):
+        rows, keys = slice(at_q, at_q + nq), slice(at_k, at_k + nk)
+        others = [torch.full_like(t, value) for t in (q, k, v)]
+        for o, t, s in zip(others, (q, k, v), (rows, keys, keys)):
+            o[s] = t[s]
+        for causal in (False, True):
+            got, lse = attention_packed(*others, cu_q.to(torch.int32), cu_k.to(torch.int32), causal=causal, return_lse=True)
+            _check_attention(got[rows], lse[rows], _attention_reference(q[rows], k[keys], v[keys], [nq], [nk], causal))
+        at_q, at_k = at_q + nq, at_k + nk
+
+
 def test_no_wait_has_run_out():
     import ctypes
     from sacq_b200 import _lib
