@@ -150,9 +150,8 @@ __device__ __noinline__ inline void redo_row(const AttnParams& a, const AttnSpli
   for (int e = 0; e < 4; ++e) {
     const int d = lane + 32 * e;
     if (d >= a.dim || d < from || d >= to) continue;
-    const float o = st.acc[e] / st.l;
-    if (part < 0) a.out[token * a.out_token + head * a.out_head + d] = float_to_bf16_bits(o);
-    else split.part_o[(((int64_t)part * a.tokens_q + token) * a.heads + head) * a.dim + d] = o;
+    if (part < 0) a.out[token * a.out_token + head * a.out_head + d] = float_to_bf16_bits(st.acc[e] / st.l);
+    else split.part_o[(((int64_t)part * a.tokens_q + token) * a.heads + head) * a.dim + d] = st.m == -INFINITY ? st.acc[e] : st.acc[e] / st.l;
   }
 }
 

@@ -351,7 +351,8 @@ attention_short_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     uint32_t odd = 0;                        // rows with a value that is not finite and keys among those multiplied that they do not see
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float inv = mine[h] > 0 ? 1.0f / l[h] : 0.f;
+      // a chunk whose keys all score -inf: its sums, zeros, as they are, since the chunks are joined with a weight of zero for it
+      const float inv = mine[h] == 0 ? 0.f : it.part >= 0 && m[h] == -INFINITY ? 1.f : 1.0f / l[h];
       bool finite = true;
       const int64_t slot = ((int64_t)max(it.part, 0) * a.tokens_q + token[h]) * a.heads + head[h];
       uint16_t* const out = a.out + (int64_t)token[h] * a.out_token + (int64_t)head[h] * a.out_head;

@@ -19,7 +19,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
   if (token >= a.tokens_q) return;
   const int sequence = sequence_of(a.cu_q, a.sequences, a.tokens_q, token);
   if (sequence < 0) return;
-  const Span sk = span_of(a.cu_k, sequence, a.tokens_k);
+  const Span sq = span_of(a.cu_q, sequence, a.tokens_q), sk = span_of(a.cu_k, sequence, a.tokens_k);
   const int chunks = chunks_of(split, (int)sk.length);
   if (chunks == 1) return;                   // written by the attention kernel
   const int64_t stride = a.tokens_q * a.heads, at = token * a.heads + head;
@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
   const int d = lane * 4;
   const float* const src = split.part_o + at * a.dim + (d < a.dim ? d : 0);
   for (int first = 0; first < chunks; first += 32) {
-    // this lane's chunk's weight: 0 where the query sees none of its keys, whose part is zeros
+    // this lane's chunk's weight: 0 where the query sees none of its keys or all of them score -inf, and the part is zeros
     const int n = min(32, chunks - first);
     const float f = lane < n ? exp2f((split.part_lse[(first + lane) * stride + at] - base) * kLog2e) : 0.f;
     for (int i = 0; i < n; i += 8) {         // eight parts are on their way at a time
@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
       }
     }
   }
-  const bool some = l != 0.f;                // a NaN is some, too
+  const bool some = a.causal ? token - sq.begin + sk.length - sq.length >= 0 : true;      // keys that the query sees: they may all score -inf
   if (d < a.dim) {
     const float inv = some ? 1.0f / l : 0.f;
     *reinterpret_cast<uint2*>(a.out + token * a.out_token + head * a.out_head + d) =

@@ -758,7 +758,8 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 #pragma unroll
           for (int e = 0; e < 64; ++e)
             if (h * 64 + e >= a.dim) o[e >> 5][e & 31] = 0u;
-        if (h == 0) inv = mine > 0 ? 1.0f / l : 0.f;
+        // a chunk whose keys all score -inf: its sums, zeros, as they are, since the chunks are joined with a weight of zero for it
+        if (h == 0) inv = mine == 0 ? 0.f : SPLIT && it.part >= 0 && m == -INFINITY ? 1.f : 1.0f / l;
         const uint64_t inv2 = f32x2(inv, inv);
         uint64_t odd2 = f32x2(0.f, 0.f);     // NaN if a value is not finite
 #pragma unroll

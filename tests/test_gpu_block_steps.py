@@ -809,6 +809,30 @@ def test_attention_of_few_queries_keeps_other_sequences_out(value, heads, kv_hea
         at_q, at_k = at_q + nq, at_k + nk
 
 
+@pytest.mark.parametrize("lq,heads,kv_heads,dim,cut", ((3, 4, 2, 128, True), (1, 1, 1, 64, True), (100, 4, 4, 128, True), (100, 4, 4, 64, True), (100, 16, 16, 64, False),
+                                                       (70, 2, 1, 36, False)))
+def test_attention_of_keys_that_score_minus_infinity(lq, heads, kv_heads, dim, cut):
+    """Keys whose scores are -inf have no weight, also where a whole chunk has no others; a row with no other key is NaN, as in the formula."""
+    from sacq_b200 import attention_packed
+    gen = _gen(14)
+    lk = 4100 if cut else 300
+    none = lk // 4 * 3
+    q = _randn(gen, lq, heads, dim).abs() + 0.125
+    k, v = (_randn(gen, lk, kv_heads, dim) for _ in range(2))
+    k[:none] = -INF
+    cu_q, cu_k = _offsets([lq]), _offsets([lk])
+    assert _cut_up(q, k, v, cu_q, cu_k) == cut
+    got, lse = attention_packed(q, k, v, cu_q, cu_k, return_lse=True)
+    _check_attention(got, lse, _attention_reference(q, k[none:], v[none:], [lq], [lk - none], False))
+    k[none:] = -INF
+    got, lse = attention_packed(q, k, v, cu_q, cu_k, return_lse=True)
+    assert bool(got.isnan().all()) and bool((lse == -INF).all() or lse.isnan().all())
+    v[5] = INF                               # a weight of zero times infinity: NaN, in whichever chunk it is
+    k[none:] = 0.0
+    got = attention_packed(q, k, v, cu_q, cu_k)
+    assert bool(got[:, :heads // kv_heads].isnan().all())
+
+
 def test_no_wait_has_run_out():
     import ctypes
     from sacq_b200 import _lib
