@@ -621,7 +621,8 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             ++no;
             tc_fence_after();
           }
-          if (__any_sync(0xffffffffu, !((high - m) * c2 <= kRescale))) {      // NaN: yes
+          // NaN: yes.  Rows behind the sequence are its neighbours' and have no say: a result's bits are its request's own
+          if (__any_sync(0xffffffffu, valid && !((high - m) * c2 <= kRescale))) {
             const float keep = m == -INFINITY ? 0.f : exp2_fast((m - high) * c2);
             m = high;
             l *= keep;

@@ -833,6 +833,24 @@ def test_attention_of_keys_that_score_minus_infinity(lq, heads, kv_heads, dim, c
     assert bool(got[:, :heads // kv_heads].isnan().all())
 
 
+@pytest.mark.parametrize("lq,lk,heads,kv_heads", (([40, 90], [700, 300], 2, 2), ([140, 3], [900, 140], 4, 2), ([40, 90], [9000, 300], 2, 2)))
+@pytest.mark.parametrize("dim", (64, 128))
+@pytest.mark.parametrize("factor", (NAN, 100.0))
+def test_attention_of_a_request_does_not_depend_on_its_neighbours_values(factor, dim, lq, lk, heads, kv_heads):
+    """To the bit: its neighbours' queries lie in the same tile."""
+    from sacq_b200 import attention_packed
+    gen = _gen(15)
+    q = _randn(gen, sum(lq), heads, dim)
+    k, v = (_randn(gen, sum(lk), kv_heads, dim) for _ in range(2))
+    cu_q, cu_k = _offsets(lq), _offsets(lk)
+    want = attention_packed(q, k, v, cu_q, cu_k, return_lse=True)
+    q[lq[0]:] *= factor
+    v[lk[0]:] *= factor
+    k[lk[0]:] *= factor
+    got = attention_packed(q, k, v, cu_q, cu_k, return_lse=True)
+    assert all(torch.equal(g[:lq[0]], w[:lq[0]]) for g, w in zip(got, want))
+
+
 def test_no_wait_has_run_out():
     import ctypes
     from sacq_b200 import _lib
