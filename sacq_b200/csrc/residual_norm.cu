@@ -255,25 +255,23 @@ __device__ __forceinline__ void norm_row(const NormParams& p, int64_t m, const R
     high = absmax_nan(high, a, b);
   });
   const float big = __uint_as_float(reduce.most(__float_as_uint(high)));
-  const float scale = big > 0.f ? big * (1.0f / 448.0f) : 1.0f;       // a NaN row keeps 1, as in quantize_rows
-  if (tid == 0) p.scale[m] = scale;
-  // h / scale as h (r1 + r2), the reciprocal in two parts: an ordinary scale is one that leaves both ordinary
-  const bool ordinary = scale > 8.3e-25f && scale < 1.2e24f;
-  const float first = ordinary ? __fdividef(1.0f, scale) : 0.f, second = fmaf(-scale, first, 1.0f) * first;
+  // scale and quotients as in quantize_rows: a NaN row keeps 1
+  const RowDivisor d = scale_of<false>(big);
+  if (tid == 0) p.scale[m] = d.s;
   uint8_t* const qrow = p.q + m * K;
-  const uint64_t r1 = f32x2(first, first), r2 = f32x2(second, second);
+  const uint64_t r1 = f32x2(d.r, d.r), r2 = f32x2(d.r2, d.r2);
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     uint32_t two[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float a, b;
-      if (ordinary) {
+      if (d.fast) {
         halves_of(quotient2(x[c][j], r1, r2), a, b);
       } else {
         halves_of(x[c][j], a, b);
-        a = __fdiv_rn(a, scale);
-        b = __fdiv_rn(b, scale);
+        a = __fdiv_rn(a, d.s);
+        b = __fdiv_rn(b, d.s);
       }
       two[j] = float2_to_e4m3x2(sat448(a), sat448(b));
     }

@@ -851,6 +851,20 @@ def test_attention_of_a_request_does_not_depend_on_its_neighbours_values(factor,
     assert all(torch.equal(g[:lq[0]], w[:lq[0]]) for g, w in zip(got, want))
 
 
+@pytest.mark.parametrize("m,k", ((40, 64), (1500, 520), (1100, 2048), (1100, 2056), (1030, 1111), (20, 6144)))
+def test_residual_norm_makes_8_bit_rows_as_the_quantizer_does(m, k):
+    """Rows that are their own shift to the bit, of maxima of any size, against quantize_rows: the same scales and bytes."""
+    from sacq_b200 import quantize_rows, residual_norm_quantize_rows
+    gen = _gen(m + k)
+    shift = _randn(gen, m, k, by=1.0) * (torch.randint(-40, 40, (m, 1), generator=gen, device="cuda").float().exp2()).to(torch.bfloat16)
+    rows = torch.randperm(m, generator=gen, device="cuda").to(torch.int32)
+    zero = torch.zeros(k, dtype=torch.bfloat16, device="cuda")
+    _, q, s = residual_norm_quantize_rows(_randn(gen, m, k), _randn(gen, m, k), zero, mod_scale=torch.zeros_like(shift), mod_shift=shift, vector_rows=rows)
+    want_q, want_s = quantize_rows(shift[rows.long()])
+    assert torch.equal(s.view(-1), want_s.view(-1))
+    assert torch.equal(q.view(torch.uint8), want_q.view(torch.uint8))
+
+
 def test_no_wait_has_run_out():
     import ctypes
     from sacq_b200 import _lib
