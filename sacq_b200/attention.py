@@ -7,13 +7,17 @@ from __future__ import annotations
 import math
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _lib
 
 
 def refuse_grad(name: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    given = [t for t in tensors if isinstance(t, torch.Tensor)]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
         raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in given):
+        raise RuntimeError(f"{name} has no forward-mode derivative: call it on the primals of dual tensors")
 
 
 def _heads(t, what: str) -> torch.Tensor:

@@ -496,8 +496,8 @@ PyObject* py_layernorm_quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n
 }
 
 // ---------------------------------------------------------------- the steps between projections
-// Whether autograd would expect a backward pass through this call: refused by the general route.
-bool wants_grad(const at::Tensor& t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
+// Whether autograd would expect a backward pass through this call, or a tangent out of it: refused by the general route.
+bool wants_grad(const at::Tensor& t) { return (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(/*level=*/0).defined(); }
 
 // bf16 [tokens, heads, dim] with unit inner stride and strides that go forwards
 const at::Tensor* heads_of(PyObject* o, int dev) {

@@ -865,6 +865,26 @@ def test_residual_norm_makes_8_bit_rows_as_the_quantizer_does(m, k):
     assert torch.equal(q.view(torch.uint8), want_q.view(torch.uint8))
 
 
+def test_steps_refuse_forward_mode_tangents():
+    import torch.autograd.forward_ad as forward_ad
+    from sacq_b200 import attention_packed, residual_norm_quantize_rows, rotary_frequencies, rotate_heads
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    q, k, cu = z(4, 4, 64), z(4, 2, 64), _offsets([4])
+    pos, (freq, _) = torch.zeros(4, dtype=torch.int32, device="cuda"), rotary_frequencies(64)
+    x, v = z(4, 64), z(64)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: attention_packed(dual(q), k, k, cu), lambda: attention_packed(q, k, dual(k), cu), lambda: attention_packed(q, k, k, cu, out=dual(z(4, 4, 64))),
+                     lambda: rotate_heads(dual(q), k, pos, freq), lambda: rotate_heads(q, dual(k), pos, freq),
+                     lambda: residual_norm_quantize_rows(dual(x), x), lambda: residual_norm_quantize_rows(x, dual(x)),
+                     lambda: residual_norm_quantize_rows(x, x, dual(v)), lambda: residual_norm_quantize_rows(x, x, gate=dual(v))):
+            with pytest.raises(RuntimeError, match="derivative"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="derivative"):
+                call()
+        attention_packed(forward_ad.unpack_dual(dual(q)).primal, k, k, cu)
+
+
 def test_no_wait_has_run_out():
     import ctypes
     from sacq_b200 import _lib
