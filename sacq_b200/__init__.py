@@ -9,7 +9,7 @@ from .packing import index_bits_for, index_window_bytes, pack_indices, pack_payl
 __all__ = [
     "PrecomputedPackedVectorCodebookLinear", "forward_shared", "linear_a8_multi", "quantize_rows", "act_quantize_rows", "modulate_quantize_rows", "layernorm_quantize_rows", "pack_indices", "unpack_indices",
     "pack_payload", "index_bits_for", "index_window_bytes", "attention_packed", "rotate_heads", "rotary_frequencies",
-    "residual_norm_quantize_rows",
+    "residual_norm_quantize_rows", "block_steps_status",
 ]
 
 
@@ -17,7 +17,7 @@ __all__ = [
 _LAZY = {
     "PrecomputedPackedVectorCodebookLinear": "linear", "forward_shared": "linear", "linear_a8_multi": "linear",
     "layernorm_quantize_rows": "activation", "modulate_quantize_rows": "activation", "act_quantize_rows": "activation",
-    "quantize_rows": "activation", "residual_norm_quantize_rows": "activation", "attention_packed": "attention",
+    "quantize_rows": "activation", "residual_norm_quantize_rows": "activation", "attention_packed": "attention", "block_steps_status": "attention",
     "rotate_heads": "rotary", "rotary_frequencies": "rotary",
 }
 

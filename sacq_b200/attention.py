@@ -4,6 +4,7 @@ The reference leaves attention to its framework; here it is one call on the rows
 produce, for requests of different lengths without padding, and for single tokens against a long past."""
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -26,6 +27,15 @@ def _heads(t, what: str) -> torch.Tensor:
     if not t.is_cuda:
         raise ValueError(f"{what} must be a CUDA tensor; there is no CPU path")
     return t
+
+
+def block_steps_status(device=None) -> int:
+    """0, or a nonzero code once a bounded wait of ``attention_packed`` or ``residual_norm_quantize_rows`` has given up on ``device`` (the
+    current one by default): what that call returned is not its result.  Synchronises the device (``sacq_block_steps_status``)."""
+    word = ctypes.c_int(0)
+    with torch.cuda.device(device):
+        _lib.check(_lib.load().sacq_block_steps_status(ctypes.byref(word)))
+    return word.value
 
 
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor | None = None, *,

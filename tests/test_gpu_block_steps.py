@@ -885,6 +885,13 @@ def test_steps_refuse_forward_mode_tangents():
         attention_packed(forward_ad.unpack_dual(dual(q)).primal, k, k, cu)
 
 
+def test_the_status_of_bounded_waits_is_read_per_device():
+    from sacq_b200 import block_steps_status
+    assert block_steps_status() == 0 and block_steps_status("cuda:0") == 0 and block_steps_status(torch.device("cuda", 0)) == 0
+    with pytest.raises((RuntimeError, AssertionError)):
+        block_steps_status(torch.cuda.device_count())
+
+
 def test_no_wait_has_run_out():
     import ctypes
     from sacq_b200 import _lib
