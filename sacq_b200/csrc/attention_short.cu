@@ -348,7 +348,7 @@ attention_short_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
       if (!ok) break;
     }
     if (warp >= 2) continue;
-    uint32_t odd = 0;                        // rows with a value that is not finite and keys among those multiplied that they do not see
+    uint32_t odd = 0;                        // which of the two rows have a value that is not finite
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       // a chunk whose keys all score -inf: its sums, zeros, as they are, since the chunks are joined with a weight of zero for it
@@ -371,19 +371,17 @@ attention_short_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         if (it.part >= 0) p.split.part_lse[slot] = le;
         else if (a.lse != nullptr) a.lse[(int64_t)token[h] * a.heads + head[h]] = le;
       }
-      // a warp multiplies 32 keys at a time, those of the last 32 that no row of the tile sees among them
-      const uint32_t bad = __ballot_sync(0xffffffffu, valid[h] && !finite && mine[h] > 0 && mine[h] < min((most + 31) & ~31, it.keys));
-#pragma unroll
-      for (int r = 0; r < 8; ++r)
-        if (bad & (0xfu << (4 * r))) odd |= 1u << (r + 8 * h);
+      if (valid[h] && !finite && mine[h] > 0) odd |= 1u << h;
     }
     __syncwarp();                            // the rows as they are lie in front of the ones made again
-    while (odd != 0) {
-      const int r = __ffs(odd) - 1, src = (r & 7) * 4, h = r >> 3;
-      odd &= odd - 1;
-      redo_row(a, p.split, it.k_row, it.kv_head, it.part, __shfl_sync(0xffffffffu, h ? token[1] : token[0], src),
-               __shfl_sync(0xffffffffu, h ? head[1] : head[0], src), __shfl_sync(0xffffffffu, h ? mine[1] : mine[0], src), out_half * DP / 2,
-               (out_half + 1) * DP / 2);
+    // a warp multiplies 32 keys at a time, those of the last 32 that no row of the tile sees among them; the first lane of four stands for a row
+    const int end = min((most + 31) & ~31, it.keys);
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t bad = __ballot_sync(0xffffffffu, (odd >> h) & 1);
+      if (bad != 0)
+        redo_rows(a, p.split, it.k_row, it.kv_head, it.part, h ? token[1] : token[0], h ? head[1] : head[0], h ? mine[1] : mine[0],
+                  (lane & 3) == 0 && (bad >> lane & 0xf) != 0, end, out_half * DP / 2, (out_half + 1) * DP / 2);
     }
   }
 }

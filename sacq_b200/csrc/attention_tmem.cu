@@ -842,18 +842,11 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       // a value that is not finite may have come in with a weight of zero: from keys that other rows of the tile see, or
       // that share an instruction with them
       __syncwarp();                          // the rows as they are lie in front of the ones made again
-      uint32_t odd = __ballot_sync(0xffffffffu, valid && !finite);
-      if (odd != 0) {
+      if (__any_sync(0xffffffffu, valid && !finite)) {
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         __syncwarp();
         const int most = seen(it, causal, min(it.q_left, (it.dual && w == 1 ? 2 : 1) * tile_tokens) - 1);
-        odd = __ballot_sync(0xffffffffu, valid && !finite && mine < min((most + 15) & ~15, it.keys));
-      }
-      while (odd != 0) {
-        const int src = __ffs(odd) - 1;
-        odd &= odd - 1;
-        redo_row(a, p.split, it.k_row, it.kv_head, SPLIT ? it.part : -1, __shfl_sync(0xffffffffu, token, src), __shfl_sync(0xffffffffu, head, src),
-                 __shfl_sync(0xffffffffu, mine, src), 0, DP);
+        redo_rows(a, p.split, it.k_row, it.kv_head, SPLIT ? it.part : -1, token, head, mine, valid && !finite, min((most + 15) & ~15, it.keys), 0, DP);
       }
     }
   }
