@@ -923,6 +923,34 @@ def test_attention_of_infinities_that_are_seen_makes_no_row_again(lengths, past,
     assert _fastest(call) <= 4 * plain
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", ((16, 8, 128), (16, 16, 64), (8, 1, 96), (24, 24, 32)))
+@pytest.mark.parametrize("causal", (False, True))
+def test_attention_of_more_items_than_the_device_has_room_for(heads, kv_heads, dim, causal):
+    """128-row tiles: CTAs take item after item, of one to nine steps of keys, lone tiles and pairs, and items that have not begun."""
+    lengths = [57 + (41 * i) % 244 for i in range(40)]
+    for at, n in ((3, 1), (7, 0), (11, 9), (20, 1100), (33, 700)):
+        lengths[at] = n
+    _attend(lengths, lengths, heads, kv_heads, dim, causal, seed=17)
+    others = [lengths[(7 * i + 5) % 40] for i in range(40)]
+    _attend(lengths, others, heads, kv_heads, dim, causal, seed=18)
+
+
+@pytest.mark.parametrize("dim", (64, 128))
+@pytest.mark.parametrize("causal", (False, True))
+def test_attention_of_more_chunks_than_the_device_has_room_for(dim, causal):
+    lq, lk = [80] * 8, [16000] + [100 + 33 * i for i in range(7)]
+    z = lambda t, h: torch.empty(t, h, dim, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    assert _cut_up(z(sum(lq), 8), z(sum(lk), 8), z(sum(lk), 8), _offsets(lq), _offsets(lk), causal)
+    _attend(lq, lk, 8, 8, dim, causal, seed=19)
+
+
+@pytest.mark.parametrize("dim", (64, 128))
+def test_attention_of_few_queries_of_more_items_than_the_device_has_room_for(dim):
+    lq, lk = [1 + i % 16 for i in range(90)], [(97 * i) % 700 for i in range(90)]
+    for causal in (False, True):
+        _attend(lq, lk, 16, 8, dim, causal, seed=20)
+
+
 def test_no_wait_has_run_out():
     import ctypes
     from sacq_b200 import _lib
