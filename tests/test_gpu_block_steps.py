@@ -951,6 +951,91 @@ def test_attention_of_few_queries_of_more_items_than_the_device_has_room_for(dim
         _attend(lq, lk, 16, 8, dim, causal, seed=20)
 
 
+def _block_reference(blk, x, lengths, causal=False, rotary=None, cross=None, modulation=None, gates=(None, None)):
+    """A block on packed rows from its own quantized linears, one at a time, and float64 norms, rotation and attention: what
+    _Block.forward states for each sequence, with gates on the attention branches."""
+    from sacq_b200 import act_quantize_rows, quantize_rows
+    bf = torch.bfloat16
+    t = x.shape[0]
+    zero = torch.zeros(blk.hidden, dtype=bf, device=x.device)
+    m = (zero,) * 4 if modulation is None else modulation.view(4, blk.hidden)         # shift, scale in front of attention; the same in front of the MLP
+
+    def rows(norm, x, shift, scale):
+        h = torch.nn.functional.layer_norm(x.double(), (blk.hidden,), None if norm.weight is None else norm.weight.double(),
+                                           None if norm.bias is None else norm.bias.double(), norm.eps)
+        return quantize_rows((h * (1 + scale.double()) + shift.double()).to(bf))
+
+    def attend(q, k, v, lq, lk, causal):
+        heads = lambda y: y.view(y.shape[0], -1, blk.head_dim)  # noqa: E731
+        return _attention_reference(heads(q), heads(k), heads(v), lq, lk, causal)[0].to(bf).view(t, blk.hidden)
+
+    def add(x, branch, gate):
+        return (x.double() + (1.0 if gate is None else gate.double()) * branch.double()).to(bf)
+
+    q, k, v = (layer.linear_a8(*rows(blk.n1, x, m[0], m[1])) for layer in (blk.q, blk.k, blk.v))
+    if rotary is not None:
+        q, k = (_rotary_reference(y.view(t, -1, blk.head_dim), *rotary, "half", 1.0)[0].to(bf).view(t, -1) for y in (q, k))
+    x = add(x, blk.o(attend(q, k, v, lengths, lengths, causal)), gates[0])
+    if cross is not None:
+        keys, values, others = cross
+        x = add(x, blk.co(attend(blk.cq.linear_a8(*rows(blk.n3, x, zero, zero)), keys, values, lengths, others, False)), gates[1])
+    up = blk.up.linear_a8(*rows(blk.n2, x, m[2], m[3]))
+    if blk.gated:
+        down = act_quantize_rows("silu_mul", blk.gate.linear_a8(*rows(blk.n2, x, m[2], m[3])), up)
+    else:
+        down = act_quantize_rows("gelu", up)
+    return blk.down.linear_a8(*down, residual=x)
+
+
+@pytest.mark.parametrize("kind", ("vision", "language", "action"))
+def test_packed_blocks_against_their_formula(kind):
+    """Each kind of block of the packed forward.  Rows that are rounded to bf16 at other places differ by 2^-10 on average, so one e4m3 value in 2^-10 / 2^-3.5
+    of its neighbour's distance becomes its neighbour: 2^-6.75 of the norm of what a linear gets, 0.023 after the six that follow
+    one another; 0.05 of what the block adds.  The same formula with a gate, a norm's vectors, the rotation, the mask or the context of another place is
+    off by twice that at least (the norm in front of the language model's attention has large weights: its scores would be too flat to tell)."""
+    from sacq_b200 import rotary_frequencies
+    from sacq_b200.policy import _Block, _Factory
+    gen = _gen(22)
+    f = _Factory(torch.device("cuda"), 5)
+    lengths = [70, 1, 33]
+    t, hidden = sum(lengths), 512
+    x = _randn(gen, t, hidden)
+    cu = _offsets(lengths)
+    given, wrong, packed = {}, [], {}
+    if kind == "vision":
+        blk = _Block(f, hidden, 8, 8, 1024, gated=False)
+        wrong = [{"lengths": [t]}]
+    elif kind == "language":
+        blk = _Block(f, hidden, 4, 2, 1024, gated=True)
+        positions = torch.cat([torch.arange(n) for n in lengths]).to(torch.int32).cuda()
+        given = {"causal": True, "rotary": (positions, rotary_frequencies(128, base=1e6)[0])}
+        packed = given
+        wrong = [{"causal": False}, {"rotary": None}, {"rotary": (positions * 2, given["rotary"][1])}]
+    else:
+        blk = _Block(f, hidden, 4, 4, 1024, gated=False, cross_dim=hidden, adaln=True)
+        blk.cv = _Factory(torch.device("cuda"), 6).linear(hidden, hidden)             # layers of one shape and factory have one payload
+        others = [20, 41, 7]
+        context = blk.cross_kv(_randn(gen, sum(others), hidden))
+        modulation, gates = _randn(gen, 4 * hidden, by=0.5), _randn(gen, 2, hidden)
+        given = {"cross": (*context, others), "modulation": modulation, "gates": gates}
+        packed = {"cross": (*context, _offsets(others)), "modulation": modulation, "gates": gates}
+        wrong = [{"gates": gates.flip(0)}, {"gates": (None, None)}, {"modulation": modulation.view(4, hidden)[[1, 0, 2, 3]]}, {"modulation": modulation.view(4, hidden)[[2, 3, 0, 1]]},
+                 {"cross": (context[1], context[0], others)}, {"cross": (*context, others[::-1])}]
+    for norm in (blk.n1, blk.n2, getattr(blk, "n3", None)):
+        if norm is not None and norm.weight is not None:
+            norm.weight.data.copy_(_randn(gen, hidden, at=2.5 if kind == "language" and norm is blk.n1 else 1.0, by=0.2))
+            norm.bias.data.copy_(_randn(gen, hidden, by=0.2))
+    with torch.no_grad():
+        got = blk.forward_packed(x, cu, **packed)
+        ref = _block_reference(blk, x, **{"lengths": lengths, **given})
+        added = (ref.double() - x.double()).norm()
+        off = lambda y: float((y.double() - ref.double()).norm() / added)  # noqa: E731
+        assert off(got) <= 0.05, off(got)
+        for w in wrong:
+            other = off(_block_reference(blk, x, **{"lengths": lengths, **given, **w}))
+            assert other > 0.1, (list(w), other)
+
+
 def test_no_wait_has_run_out():
     import ctypes
     from sacq_b200 import _lib
