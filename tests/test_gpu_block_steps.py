@@ -1036,6 +1036,60 @@ def test_packed_blocks_against_their_formula(kind):
             assert other > 0.1, (list(w), other)
 
 
+def _tail(gen, tokens, last, heads, dim):
+    """[tokens, heads, dim] of which the last rows are made; more than 2^31 elements."""
+    x = torch.empty(tokens, heads, dim, dtype=torch.bfloat16, device="cuda")
+    assert x.numel() > 2 ** 31
+    x[-last:] = _randn(gen, last, heads, dim)
+    return x
+
+
+@pytest.mark.parametrize("lq,heads,dim", ((200, 16, 128), (5, 16, 128), (20, 16, 40), (20, 16, 36)))
+def test_attention_of_keys_behind_two_to_the_31_elements(lq, heads, dim):
+    from sacq_b200 import attention_packed
+    gen = _gen(23)
+    tokens, last = 2_100_003, 700
+    q = _randn(gen, lq, heads, dim)
+    k, v = (_tail(gen, tokens, last, 8, 128)[..., :dim] for _ in range(2))
+    cu_k = torch.tensor([tokens - last, tokens], dtype=torch.int32, device="cuda")
+    got, lse = attention_packed(q, k, v, _offsets([lq]), cu_k, causal=True, return_lse=True)
+    _check_attention(got, lse, _attention_reference(q, k[-last:], v[-last:], [lq], [last], True))
+    # queries and results as far out, the last of their keys with values of no use
+    v[-1] = NAN
+    far = _tail(gen, 1_100_000, lq, heads, 128)
+    far[-lq:, :, :dim] = q
+    out = torch.empty_like(far)[..., :dim]
+    cu_q = torch.tensor([far.shape[0] - lq, far.shape[0]], dtype=torch.int32, device="cuda")
+    got, lse = attention_packed(far[..., :dim], k, v, cu_q, cu_k, causal=True, out=out, return_lse=True)
+    _check_attention(got[-lq:-1], lse[-lq:-1], tuple(x[:-1] for x in _attention_reference(q, k[-last:], v[-last:].nan_to_num(0.0), [lq], [last], True)))
+    assert bool(got[-1].isnan().all())
+
+
+def test_rotary_and_norms_behind_two_to_the_31_elements():
+    from sacq_b200 import residual_norm_quantize_rows, rotary_frequencies, rotate_heads
+    gen = _gen(24)
+    tokens, last = 1_050_000, 1500
+    q = _tail(gen, tokens, last, 16, 128)
+    pos, (freq, _) = torch.arange(tokens, device="cuda"), rotary_frequencies(128)
+    for layout, part in (("half", slice(0, 128)), ("interleaved", slice(0, 128)), ("half", slice(1, 128))):
+        f = freq if part.start == 0 else rotary_frequencies(40)[0]
+        want = rotate_heads(q[-last:, :, part], None, pos[-last:], f, layout=layout)[0]
+        assert torch.equal(rotate_heads(q[..., part], None, pos, f, layout=layout)[0][-last:], want)
+    x = q.view(tokens, 2048)
+    gate = _randn(gen, 3, 2048)
+    rows = (torch.arange(tokens, device="cuda") % 3).to(torch.int32)
+    kw = lambda s: dict(gate=gate, vector_rows=rows[s], return_normalized=True)  # noqa: E731
+    got = residual_norm_quantize_rows(x, x, **kw(slice(None)))
+    assert _same([t[-last:] for t in got], residual_norm_quantize_rows(x[-last:], x[-last:], **kw(slice(tokens - last, None))))
+    del got
+    odd = x[:, :2047]                        # rows that are 16-byte aligned and of odd length: elements one by one
+    got = residual_norm_quantize_rows(odd, odd, quantize=False)
+    assert _same([t[-last:] for t in got], residual_norm_quantize_rows(odd[-last:], odd[-last:], quantize=False))
+    few = x.view(-1, 8192)                   # wide rows
+    got = residual_norm_quantize_rows(few, few)
+    assert _same([t[-last // 4:] for t in got], [t[-last // 4:] for t in residual_norm_quantize_rows(few[-1100:], few[-1100:])])
+
+
 def test_no_wait_has_run_out():
     import ctypes
     from sacq_b200 import _lib
