@@ -53,8 +53,8 @@ __device__ __forceinline__ int sequence_of(const int32_t* cu_q, int sequences, i
   return -1;
 }
 
-// One query row by one warp, key after key with a running maximum: lane l holds elements l, l + 32, ...  Returns the
-// row's 1 / sum and leaves the sums in acc.
+// One query row by one warp, key after key with a running maximum: lane l holds elements l, l + 32, ... of the weighted sum in acc, every
+// lane the maximum m and the sum of weights l.
 template <int E>
 struct RowState {
   float acc[E];
@@ -246,7 +246,6 @@ AttnSplit attention_chunks(const AttnParams& a, int64_t chunk, void* workspace);
 int64_t attention_split_bytes(const AttnParams& a, const AttnSplit& split);
 int attention_tensor_maps(const AttnParams& a, int q_box_heads, int q_box_tokens, int k_box_tokens, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v);
 int attention_out_map(const AttnParams& a, int box_heads, int box_tokens, CUtensorMap* out);
-int device_sms();
 
 // Tensor cores by tcgen05: tiles of 128 query rows.
 AttnSplit attention_tmem_split(const AttnParams& p, void* workspace);

@@ -860,7 +860,7 @@ attention_tmem_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 
 struct Tiles {
   int pack_log2, groups;
-  int64_t items, per_sequence;
+  int64_t items;
 };
 Tiles tiles_of(const AttnParams& a) {
   Tiles t = {};
@@ -870,7 +870,6 @@ Tiles tiles_of(const AttnParams& a) {
   const int64_t pair_tokens = 2 * (kTile >> t.pack_log2);
   const int64_t pairs = a.tokens_q / pair_tokens + (a.tokens_q < a.sequences ? a.tokens_q : a.sequences);   // at most
   t.items = pairs * t.groups;
-  t.per_sequence = (pairs + a.sequences - 1) / a.sequences * t.groups;
   return t;
 }
 

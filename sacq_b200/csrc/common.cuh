@@ -69,6 +69,7 @@ inline sacq_layer whole_layer(const sacq_layer* L) {
 int set_error(int code, const char* fmt, ...);
 int cuda_fail(cudaError_t e, const char* what);
 void count_launch(int n = 1);
+int device_sms();                          // of the current device (attention_split.cu)
 
 #define SACQ_CUDA_TRY(expr)                                  \
   do {                                                       \

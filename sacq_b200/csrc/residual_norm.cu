@@ -579,7 +579,7 @@ int launch_residual_norm(const sacq_residual_norm_desc& d, cudaStream_t s) {
     if (fit > row_warps(per)) fit = row_warps(per);
     threads = (unsigned)fit * 32;
     smem = (size_t)(fit * (2 + own) + all) * K * 2;
-    if (grid > 148) grid = 148;
+    if (grid > device_sms()) grid = device_sms();
   } else if (many) {
     // up to 4 chunks a thread, as many as leave the fewest elements that are not there; where there are none, nothing is checked
     const int64_t pieces = (chunks + 31) / 32, pieces4 = (pieces + 3) / 4;
@@ -597,7 +597,7 @@ int launch_residual_norm(const sacq_residual_norm_desc& d, cudaStream_t s) {
     int64_t fit = (int64_t)(224 * 1024) / (int64_t)(smem + 2048);
     if (fit > 1024 / threads) fit = 1024 / threads;
     if (fit < 1) fit = 1;
-    if (grid > fit * 148) grid = fit * 148;
+    if (grid > fit * device_sms()) grid = fit * device_sms();
   } else {
     threads = (unsigned)(chunks >= 1024 ? 1024 : (chunks + 31) / 32 * 32);
     per = (int)((chunks + threads - 1) / threads);

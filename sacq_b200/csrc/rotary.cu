@@ -4,8 +4,9 @@
 // ("half") or (x[2i], x[2i + 1]) ("interleaved").
 //
 // Angles: a position of 10^6 times a frequency near 1 is right to 0.06 radians in fp32, so the product is made in
-// double, in turns (inv_freq / 2 pi), reduced to half a turn either way there, and only then rounded: the
-// rounding that is left is 2^-26 turns.  They are the same for all heads, so a CTA makes those of its tokens once, in
+// double, in turns (inv_freq / 2 pi), reduced to half a turn either way there, and only then rounded, to 2^-26 turns.
+// The quotient, the product and the constant are rounded to 53 bits: 3 x 2^-53 of the angle, which is less than that up to
+// angles of 2^28 radians and 2.9e-6 radians at 2^33.  They are the same for all heads, so a CTA makes those of its tokens once, in
 // shared memory, between its loads and its stores.
 //
 // Bound by memory: 4 bytes per element.  A thread has one place in a token (16-byte chunks, of "half" both of a pair) and takes it in
@@ -26,11 +27,11 @@ struct RotaryParams {
   const void* positions;
   const double* inv_freq;
   int64_t tokens;
-  int dim, half;                                // head dim; rotated pairs
   int per_head;                                 // units of a head: turned ones first, then copied ones
   int turned;
   int per_token;                                // units of a token, both tensors
   int per_cta;                                  // tokens of a CTA, up to kTokens
+  int half;                                     // rotated pairs
   float amplitude;
   bool wide_positions;
 };
@@ -184,7 +185,6 @@ int launch_rotate_heads(const sacq_rotary_desc& d, cudaStream_t s) {
   p.positions = d.positions;
   p.inv_freq = d.inv_freq;
   p.tokens = d.tokens;
-  p.dim = d.head_dim;
   p.half = d.rotary_dim / 2;
   p.amplitude = d.amplitude;
   p.wide_positions = d.position_bytes == 8;
@@ -193,7 +193,7 @@ int launch_rotate_heads(const sacq_rotary_desc& d, cudaStream_t s) {
   p.per_head = p.turned + (vec ? (d.head_dim - d.rotary_dim) / 8 : d.head_dim - d.rotary_dim);
   p.per_token = p.per_head * (d.q.heads + d.k.heads);
   // few tokens are spread over the SMs
-  const int64_t share = d.tokens / 148;
+  const int64_t share = d.tokens / device_sms();
   p.per_cta = share < 1 ? 1 : share < kTokens ? (int)share : kTokens;
   const int room = 48 * 1024 / (int)sizeof(float2) / p.half;
   if (p.per_cta > room) p.per_cta = room;

@@ -74,8 +74,8 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     ``q``, ``k`` (or ``None``): bf16 ``[tokens, heads, head_dim]``, any strides with a unit inner one.  ``positions``: int32 or int64
     ``[tokens]``; ``inv_freq``: float64 ``[rotary_dim / 2]`` (``rotary_frequencies``); ``rotary_dim`` is at most ``head_dim`` and what lies behind it
     is copied.  ``layout``: ``"half"`` pairs element ``i`` with ``i + rotary_dim / 2``, ``"interleaved"`` ``2 i`` with ``2 i + 1``.
-    ``out=(q_out, k_out)`` receives the results; ``out=(q, k)`` turns in place, views of one fused buffer too.  Angles are made in double: positions of any size are as exact as
-    small ones."""
+    ``out=(q_out, k_out)`` receives the results; ``out=(q, k)`` turns in place, views of one fused buffer too.  Angles are made in double and reduced there: right to 2e-7
+    radians up to 2^28 radians, to 3 x 2^-53 of the angle beyond (3e-6 at 2^33); positions above 2^53 are rounded."""
     if layout not in _LAYOUTS:
         raise ValueError(f"unknown layout {layout!r}")
     q_out, k_out = (None, None) if out is None else out
