@@ -387,8 +387,9 @@ typedef struct sacq_attention_desc {
 /* Softmax attention of packed sequences of different lengths, query heads in groups of heads / kv_heads:
  *   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j)  over the keys that the query sees
  * Scores, sums and the running maximum are fp32.  A query that sees no key has out = 0 and lse = -inf.  Offsets that leave the
- * tensors are cut to them, a sequence that ends in front of its beginning is empty, and sequences may not share queries.  What lies
- * in keys and values that a query does not see, NaN included, does not reach its output. */
+ * tensors are cut to them, a sequence that ends in front of its beginning is empty, and sequences may not share queries.  Room behind a
+ * past is a sequence without queries.  What lies in keys and values that a query does not see, NaN included, does not reach its output,
+ * nor do other sequences' values change its bits. */
 SACQ_API int sacq_attention_packed(const sacq_attention_desc* desc, void* stream);
 SACQ_API int64_t sacq_attention_workspace_bytes(const sacq_attention_desc* desc);
 /* Reads the current device's status word of these kernels (synchronises the device): 0, or a nonzero code written by one

@@ -51,7 +51,9 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     ``causal``: query ``i`` of ``n`` sees keys up to ``i + (keys - n)``, so that new tokens behind a longer past see all of it.
     ``scale`` defaults to ``head_dim ** -0.5``.  Returns ``out`` like ``q`` (and with ``return_lse`` the fp32
     ``[tokens_q, heads]`` logarithm of each row's sum of exponentials).  A query that sees no key gets zeros and ``-inf``.
-    Rows outside of every sequence are not written.  The call does not read the offsets on the host and can be captured in a
+    Rows outside of every sequence are not written.  Offsets may go down: such a sequence is empty.  Room behind a past in a cache is a sequence
+    without queries (``cu_q = [0, 1, 1, 2, 2]``, ``cu_k = [0, 500, 4096, 4696, 8192]``).  Kernel and chunks of keys are chosen from the averages of the call: a batch
+    of very unlike sequences may be faster as two calls.  The call does not read the offsets on the host and can be captured in a
     CUDA graph."""
     made = _lib.native().attention_packed(q, k, v, cu_q, cu_k, bool(causal), scale, out, bool(return_lse))
     if made is not None:

@@ -1090,6 +1090,22 @@ def test_rotary_and_norms_behind_two_to_the_31_elements():
     assert _same([t[-last // 4:] for t in got], [t[-last // 4:] for t in residual_norm_quantize_rows(few[-1100:], few[-1100:])])
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,new", ((16, 8, 128, 1), (4, 4, 64, 40), (2, 1, 36, 3)))
+def test_attention_of_a_cache_with_room_behind_each_past(heads, kv_heads, dim, new):
+    """The room is a sequence without queries, and may hold anything."""
+    from sacq_b200 import attention_packed
+    gen = _gen(25)
+    room, pasts = 4096, [500, 600, 4096, 41]
+    q = _randn(gen, new * len(pasts), heads, dim)
+    cache = [torch.full((room * len(pasts), kv_heads, dim), NAN, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    rows = torch.cat([torch.arange(n) + i * room for i, n in enumerate(pasts)]).cuda()
+    for t in cache:
+        t[rows] = _randn(gen, sum(pasts), kv_heads, dim)
+    cu_q, cu_k = _offsets([n for _ in pasts for n in (new, 0)]), _offsets([n for past in pasts for n in (past, room - past)])
+    got, lse = attention_packed(q, *cache, cu_q, cu_k, causal=True, return_lse=True)
+    _check_attention(got, lse, _attention_reference(q, *(t[rows] for t in cache), [new] * len(pasts), pasts, True))
+
+
 def test_no_wait_has_run_out():
     import ctypes
     from sacq_b200 import _lib
