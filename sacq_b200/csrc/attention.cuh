@@ -121,7 +121,8 @@ __device__ __forceinline__ int chunks_of(const AttnSplit& s, int keys) {
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
-// Waits of these kernels: a warp that makes 32 rows again (redo_rows) is at it for 60 clocks a row and key, others wait meanwhile.
+// Waits of these kernels: a warp that makes 32 rows again (redo_rows) is at it for 60 clocks a row and key, a microsecond a key, and others wait meanwhile:
+// long enough for 10 million keys.
 constexpr uint64_t kWaitNs = 10000000000ull;
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
